@@ -17,6 +17,9 @@ ADD, SUB, MUL, DIV = 0, 1, 2, 3
 RELU, LEAKY_RELU, GELU, SIGMOID, TANH = 0, 1, 2, 3, 4
 REDUCE_SUM, REDUCE_MEAN, REDUCE_MAX = 0, 1, 2
 TREE_INTERLEAVE, TREE_ADDRESS = 0, 1
+F32, F16, BF16 = 0, 1, 2
+NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
+GATE_PLAIN, GATE_SIGMOID, GATE_TANH = 0, 1, 2
 
 _vp, _i64, _int, _f32, _f64, _sz = C.c_void_p, C.c_int64, C.c_int, C.c_float, C.c_double, C.c_size_t
 _pi64 = C.POINTER(C.c_int64)
@@ -63,6 +66,19 @@ PROTOTYPES = {
     "fdl_transpose_f32": (_int, [_vp, _vp, _i64, _vp]),
     "fdl_uniform_f32": (_int, [_vp, _i64, _f32, _f32, C.c_uint64, _vp]),
     "fdl_normal_f32": (_int, [_vp, _i64, _f32, _f32, C.c_uint64, _vp]),
+    "fdl_distill_topk": (_int, [_vp, _i64, _int, _vp, _int, _vp, _vp, _vp, _i64, _i64, _i64, _f32, _f32, _vp, _vp, _vp,
+                                _vp]),
+    "fdl_distill_topk_backward": (_int, [_vp, _i64, _int, _vp, _int, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _f32,
+                                         _f32, _vp, _i64, _vp]),
+    "fdl_distill_topk_with_grad": (_int, [_vp, _i64, _int, _vp, _int, _vp, _vp, _vp, _i64, _i64, _i64, _f32, _f32, _vp,
+                                          _vp, _vp, _vp, _i64, _vp]),
+    "fdl_norm_residual": (_int, [_vp, _vp, _vp, _i64, _int, _int, _vp, _vp, _int, _vp, _vp, _vp, _vp, _vp, _i64, _i64,
+                                 _f32, _f32, _f32, _int, _vp]),
+    "fdl_norm_residual_backward_scratch_bytes": (_sz, [_i64, _i64, _i64]),
+    "fdl_norm_residual_backward": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _int, _int, _vp, _vp, _int, _vp, _vp, _vp,
+                                          _vp, _vp, _vp, _vp, _vp, _i64, _i64, _f32, _f32, _int, _vp, _sz, _vp]),
+    "fdl_verify_draft": (_int, [_vp, _i64, _i64, _vp, _i64, _i64, _int, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _vp,
+                                _vp]),
     "fdl_host_binary_f32": (_int, [_vp, _vp, _vp, _i64, _int]),
     "fdl_host_unary_f32": (_int, [_vp, _vp, _i64, _int, _f32]),
     "fdl_host_mul_add_relu_f32": (_int, [_vp, _vp, _vp, _vp, _i64]),
@@ -335,6 +351,228 @@ def sum_trace() -> list:
 
 def take_device_error() -> None:
     check(lib().fdl_take_device_error(), "device-side wait")
+
+
+# ---- training a model from a teacher, serving with a draft model ---------------------------------------
+#
+# 32-bit, 16-bit float and bfloat16 tensors on the current device; results go to new tensors (scratch
+# too, so that a captured call replays on memory of its own).
+
+
+_dtype_codes = None
+
+
+def _dtype_code(t, what):
+    global _dtype_codes
+    if _dtype_codes is None:
+        import torch
+        _dtype_codes = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+    code = _dtype_codes.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{what}: expected float32, float16 or bfloat16, got {t.dtype}")
+    return code
+
+
+def _here(t, what, shape=None, dtype=None, contiguous=True):
+    """`t`, if it is a tensor on the current CUDA device of this shape and type."""
+    import torch
+    if not t.is_cuda or t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{what}: expected a tensor on the current CUDA device, got {t.device}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    if dtype is not None and t.dtype != dtype:
+        raise ValueError(f"{what}: expected dtype {dtype}, got {t.dtype}")
+    if contiguous and not t.is_contiguous():
+        raise ValueError(f"{what}: expected a contiguous tensor")
+    return t
+
+
+def _rows_of(t, what):
+    """Row stride of a matrix whose rows are contiguous and do not overlap."""
+    rows, cols = t.shape
+    if (cols > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < cols):
+        raise ValueError(f"{what}: expected contiguous rows that do not overlap, got strides {t.stride()}")
+    return max(t.stride(0), cols) if rows > 1 else cols
+
+
+def _distill_args(where, logits, teacher, index, teacher_lse, row_weight, temperature, scale):
+    import torch
+    if logits.dim() != 2 or index.dim() != 2 or index.shape[0] != logits.shape[0]:
+        raise ValueError(f"{where}: expected logits [rows, vocab] and index [rows, k]")
+    rows, vocab = logits.shape
+    _here(logits, f"{where}: logits", contiguous=False)
+    _here(index, f"{where}: index", dtype=torch.int64)
+    _here(teacher, f"{where}: teacher", index.shape)
+    if teacher_lse is not None:
+        _here(teacher_lse, f"{where}: teacher_lse", (rows,), torch.float32)
+    if row_weight is not None:
+        _here(row_weight, f"{where}: row_weight", (rows,), torch.float32)
+    if scale is None:
+        scale = 1.0 / max(rows, 1)
+    head = (_ptr(logits), _rows_of(logits, f"{where}: logits"), _dtype_code(logits, where), _ptr(teacher),
+            _dtype_code(teacher, where), _ptr(index), _ptr(teacher_lse), _ptr(row_weight))
+    return head, (rows, vocab, index.shape[1], temperature, scale)
+
+
+def _grad_for(where, logits, out):
+    import torch
+    if out is None:
+        return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device), logits.shape[1]
+    _here(out, f"{where}: out", logits.shape, logits.dtype, contiguous=False)
+    return out, _rows_of(out, f"{where}: out")
+
+
+def distill_topk(logits, teacher, index, teacher_lse=None, row_weight=None, temperature=1.0, scale=None):
+    """Distillation loss on the teacher's k highest logits: (loss [1], row_loss [rows], row_stats [rows, 2]).
+
+    logits [rows, vocab] (rows may be padded), teacher and index (int64) [rows, k]; an index outside
+    [0, vocab) is padding.  scale: default 1 / rows (the mean).  row_stats goes to distill_topk_backward."""
+    import torch
+    head, sizes = _distill_args("distill_topk", logits, teacher, index, teacher_lse, row_weight, temperature, scale)
+    loss = torch.empty(1, dtype=torch.float32, device=logits.device)
+    row_loss = torch.empty(sizes[0], dtype=torch.float32, device=logits.device)
+    stats = torch.empty((sizes[0], 2), dtype=torch.float32, device=logits.device)
+    check(lib().fdl_distill_topk(*head, *sizes, _ptr(loss), _ptr(row_loss), _ptr(stats), _stream()), "fdl_distill_topk")
+    return loss, row_loss, stats
+
+
+def distill_topk_backward(logits, teacher, index, row_stats, teacher_lse=None, row_weight=None, temperature=1.0,
+                          scale=None, grad_loss=None, out=None):
+    """Gradient of grad_loss * loss in the logits' type; out may be `logits` itself."""
+    import torch
+    where = "distill_topk_backward"
+    head, sizes = _distill_args(where, logits, teacher, index, teacher_lse, row_weight, temperature, scale)
+    _here(row_stats, f"{where}: row_stats", (sizes[0], 2), torch.float32)
+    if grad_loss is not None:
+        _here(grad_loss, f"{where}: grad_loss", dtype=torch.float32)
+        if grad_loss.numel() != 1:
+            raise ValueError(f"{where}: grad_loss: expected one value")
+    grad, stride = _grad_for(where, logits, out)
+    check(lib().fdl_distill_topk_backward(*head, _ptr(row_stats), _ptr(grad_loss), *sizes, _ptr(grad), stride, _stream()),
+          "fdl_distill_topk_backward")
+    return grad
+
+
+def distill_topk_with_grad(logits, teacher, index, teacher_lse=None, row_weight=None, temperature=1.0, scale=None,
+                           out=None):
+    """(loss [1], row_loss [rows], gradient of the loss); out may be `logits` itself."""
+    import torch
+    where = "distill_topk_with_grad"
+    head, sizes = _distill_args(where, logits, teacher, index, teacher_lse, row_weight, temperature, scale)
+    loss = torch.empty(1, dtype=torch.float32, device=logits.device)
+    row_loss = torch.empty(sizes[0], dtype=torch.float32, device=logits.device)
+    stats = torch.empty((sizes[0], 2), dtype=torch.float32, device=logits.device)
+    grad, stride = _grad_for(where, logits, out)
+    check(lib().fdl_distill_topk_with_grad(*head, *sizes, _ptr(loss), _ptr(row_loss), _ptr(stats), _ptr(grad), stride,
+                                           _stream()), "fdl_distill_topk_with_grad")
+    return loss, row_loss, grad
+
+
+def _norm_weights(where, cols, **weights):
+    import torch
+    for name, w in weights.items():
+        if w is not None:
+            _here(w, f"{where}: {name}", (cols,), torch.float32)
+
+
+def norm_residual(x, h, post=NORM_RMS, pre=NORM_RMS, gate=None, gate_act=GATE_PLAIN, post_gamma=None, post_beta=None,
+                  pre_gamma=None, pre_beta=None, residual_scale=1.0, block_scale=1.0, eps=1e-5, out=None, out_n=None):
+    """y = residual_scale * x + block_scale * act(gate) * norm_post(h) and n = norm_pre(y): (y, n, stats [rows, 4]).
+
+    gate: [gate_rows, cols], gate_rows a divisor of rows.  n is None with pre=NORM_NONE.  out may be x, out_n h."""
+    import torch
+    where = "norm_residual"
+    if x.dim() != 2:
+        raise ValueError(f"{where}: expected [rows, cols]")
+    rows, cols = x.shape
+    _here(x, f"{where}: x")
+    _here(h, f"{where}: h", (rows, cols), x.dtype)
+    gate_rows = 0
+    if gate is not None:
+        gate_rows = gate.shape[0]
+        _here(gate, f"{where}: gate", (gate_rows, cols), x.dtype)
+    _norm_weights(where, cols, post_gamma=post_gamma, post_beta=post_beta, pre_gamma=pre_gamma, pre_beta=pre_beta)
+    y = torch.empty_like(x) if out is None else _here(out, f"{where}: out", (rows, cols), x.dtype)
+    n = None
+    if pre != NORM_NONE:
+        n = torch.empty_like(x) if out_n is None else _here(out_n, f"{where}: out_n", (rows, cols), x.dtype)
+    stats = torch.empty((rows, 4), dtype=torch.float32, device=x.device)
+    check(lib().fdl_norm_residual(_ptr(x), _ptr(h), _ptr(gate), gate_rows, gate_act, post, _ptr(post_gamma),
+                                  _ptr(post_beta), pre, _ptr(pre_gamma), _ptr(pre_beta), _ptr(y), _ptr(n), _ptr(stats),
+                                  rows, cols, residual_scale, block_scale, eps, _dtype_code(x, where), _stream()),
+          "fdl_norm_residual")
+    return y, n, stats
+
+
+def norm_residual_backward(dy, dn, y, h, stats, post=NORM_RMS, pre=NORM_RMS, gate=None, gate_act=GATE_PLAIN,
+                           post_gamma=None, post_beta=None, pre_gamma=None, residual_scale=1.0, block_scale=1.0,
+                           want_post_beta=False, want_pre_beta=False):
+    """Gradients of norm_residual as a dict: x, h, gate, post_gamma, post_beta, pre_gamma, pre_beta (None where there
+    is nothing to learn).  dy or dn may be None."""
+    import torch
+    where = "norm_residual_backward"
+    if h.dim() != 2:
+        raise ValueError(f"{where}: expected [rows, cols]")
+    rows, cols = h.shape
+    _here(h, f"{where}: h")
+    for name, t in (("dy", dy), ("dn", dn), ("y", y)):
+        if t is not None:
+            _here(t, f"{where}: {name}", (rows, cols), h.dtype)
+    _here(stats, f"{where}: stats", (rows, 4), torch.float32)
+    gate_rows = 0
+    if gate is not None:
+        gate_rows = gate.shape[0]
+        _here(gate, f"{where}: gate", (gate_rows, cols), h.dtype)
+    _norm_weights(where, cols, post_gamma=post_gamma, post_beta=post_beta, pre_gamma=pre_gamma)
+    code = _dtype_code(h, where)
+
+    def sums(wanted):
+        return torch.empty(cols, dtype=torch.float32, device=h.device) if wanted else None
+
+    out = {"x": torch.empty_like(h), "h": torch.empty_like(h), "gate": None if gate is None else torch.empty_like(gate),
+           "post_gamma": sums(post_gamma is not None), "post_beta": sums(want_post_beta),
+           "pre_gamma": sums(pre_gamma is not None), "pre_beta": sums(want_pre_beta)}
+    bytes_ = lib().fdl_norm_residual_backward_scratch_bytes(rows, cols, gate_rows)
+    scratch = torch.empty(bytes_, dtype=torch.uint8, device=h.device)
+    check(lib().fdl_norm_residual_backward(
+        _ptr(dy), _ptr(dn), _ptr(y), _ptr(h), _ptr(stats), _ptr(gate), gate_rows, gate_act, post, _ptr(post_gamma),
+        _ptr(post_beta), pre, _ptr(pre_gamma), _ptr(out["x"]), _ptr(out["h"]), _ptr(out["gate"]), _ptr(out["post_gamma"]),
+        _ptr(out["post_beta"]), _ptr(out["pre_gamma"]), _ptr(out["pre_beta"]), rows, cols, residual_scale, block_scale,
+        code, _ptr(scratch), bytes_, _stream()), "fdl_norm_residual_backward")
+    return out
+
+
+def verify_draft(target, draft_tokens, accept_u, sample_u, draft=None, draft_len=None):
+    """Drafted tokens against the target's probabilities: (tokens [batch, drafted + 1], accepted [batch]), int64.
+
+    target [batch, drafted + 1, vocab], draft [batch, drafted, vocab] or None (a draft that is certain of its
+    tokens), draft_tokens (int64) and accept_u [batch, drafted], sample_u [batch], draft_len (int64) [batch]."""
+    import torch
+    where = "verify_draft"
+    if target.dim() != 3 or draft_tokens.dim() != 2:
+        raise ValueError(f"{where}: expected target [batch, drafted + 1, vocab] and draft_tokens [batch, drafted]")
+    batch, drafted = draft_tokens.shape
+    vocab = target.shape[2]
+    _here(target, f"{where}: target", (batch, drafted + 1, vocab), contiguous=False)
+    _here(draft_tokens, f"{where}: draft_tokens", dtype=torch.int64)
+    _here(accept_u, f"{where}: accept_u", (batch, drafted), torch.float32)
+    _here(sample_u, f"{where}: sample_u", (batch,), torch.float32)
+    if draft_len is not None:
+        _here(draft_len, f"{where}: draft_len", (batch,), torch.int64)
+    strides = [0, 0]
+    if draft is not None:
+        _here(draft, f"{where}: draft", (batch, drafted, vocab), target.dtype, contiguous=False)
+        strides = draft.stride()[:2]
+    for t in (target, draft):
+        if t is not None and vocab > 1 and t.stride(2) != 1:
+            raise ValueError(f"{where}: expected a contiguous last dimension, got strides {t.stride()}")
+    tokens = torch.empty((batch, drafted + 1), dtype=torch.int64, device=target.device)
+    accepted = torch.empty(batch, dtype=torch.int64, device=target.device)
+    check(lib().fdl_verify_draft(_ptr(target), target.stride(0), target.stride(1), _ptr(draft), strides[0], strides[1],
+                                 _dtype_code(target, where), _ptr(draft_tokens), _ptr(draft_len), _ptr(accept_u),
+                                 _ptr(sample_u), batch, drafted, vocab, _ptr(tokens), _ptr(accepted), _stream()),
+          "fdl_verify_draft")
+    return tokens, accepted
 
 
 # ---- host-buffer entry points (torch CPU tensors, ideally pinned) ------------------------------

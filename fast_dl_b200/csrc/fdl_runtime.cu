@@ -145,7 +145,7 @@ void reset_workspace_counters() {
 
 extern "C" {
 
-int fdl_version(void) { return 1001; }
+int fdl_version(void) { return 1002; }
 
 const char* fdl_error_string(int status) {
     switch (status) {

@@ -74,6 +74,17 @@ enum fdl_reduce_op { FDL_REDUCE_SUM = 0, FDL_REDUCE_MEAN = 1, FDL_REDUCE_MAX = 2
  * (include/dl/kernels/reduction.hpp:7-10). */
 enum fdl_block_tree { FDL_TREE_INTERLEAVE = 0, FDL_TREE_ADDRESS = 1 };
 
+/* Element type of the operators that take 32-bit or 16-bit tensors; FDL_F32 and FDL_F16 equal
+ * dl::DType (include/dl/core/DType.hpp), FDL_BF16 has no counterpart there. */
+enum fdl_dtype { FDL_F32 = 0, FDL_F16 = 1, FDL_BF16 = 2 };
+
+/* Normalisation selector of fdl_norm_residual: none, v / sqrt(mean(v^2) + eps), or
+ * (v - mean) / sqrt(mean((v - mean)^2) + eps). */
+enum fdl_norm_kind { FDL_NORM_NONE = 0, FDL_NORM_RMS = 1, FDL_NORM_LAYER = 2 };
+
+/* What fdl_norm_residual applies to its gate. */
+enum fdl_gate_act { FDL_GATE_PLAIN = 0, FDL_GATE_SIGMOID = 1, FDL_GATE_TANH = 2 };
+
 /* ---- runtime -------------------------------------------------------------------- */
 
 /* Library ABI version: major*1000 + minor. */
@@ -388,6 +399,105 @@ int fdl_transpose_f32(const float* in, float* out, int64_t n, void* stream);
  * src/kernels/cuda/random.cu:7-56). */
 int fdl_uniform_f32(float* data, int64_t n, float low, float high, uint64_t seed, void* stream);
 int fdl_normal_f32(float* data, int64_t n, float mean, float stddev, uint64_t seed, void* stream);
+
+/* ---- training a model from a teacher, serving with a draft model (no counterpart in the reference) ----
+ *
+ * These entry points take tensors of the type `dtype` (enum fdl_dtype); gamma, beta, statistics,
+ * losses and random numbers are float.  Arithmetic is in 32 bits or more, a result of 16 bits is
+ * rounded once, to nearest even.  They use no library workspace: calls on different streams may
+ * overlap, and a captured call holds on to nothing but the caller's buffers. */
+
+/* Distillation from the teacher's k highest logits.  logits: [rows, vocab] of the student, rows
+ * `logits_stride` elements apart (>= vocab; columns beyond vocab are neither read nor written);
+ * teacher: [rows, k] values of type teacher_dtype, index: [rows, k] their columns.  An entry counts
+ * if its index is in [0, vocab) and its value is a number above -inf; the others (padding: index -1)
+ * are skipped whatever their value.  With p_j = exp(teacher_j / T) over the sum of them -- or, where
+ * teacher_lse[rows] is given, p_j = exp(teacher_j / T - teacher_lse), the teacher's own probability,
+ * with log sum exp of ALL its logits / T -- and q = softmax(logits / T):
+ *   row_loss[r] = sum_j p_j (log p_j - log q[index_j]),  loss[0] = scale * sum_r row_weight_r * row_loss_r.
+ * A column may be named by several entries.  A row of weight 0, or in which no entry counts, is left
+ * out: its loss is 0 and its logits are not read.  row_weight NULL: 1 for each row.  A student logit
+ * of -inf at a place where p_j > 0 makes the row's loss +inf; a row of nothing but -inf, and NaN or
+ * +inf among its logits, make it NaN.  row_stats: [rows, 2], the row's largest logit m and
+ * sum exp((logits - m) / T) (0, 0 for a row left out); the backward call takes it.
+ * k <= 1024, vocab < 2^31 - 65536, rows < 2^31.  Deterministic. */
+int fdl_distill_topk(const void* logits, int64_t logits_stride, int dtype, const void* teacher,
+                     int teacher_dtype, const int64_t* index, const float* teacher_lse,
+                     const float* row_weight, int64_t rows, int64_t vocab, int64_t k,
+                     float temperature, float scale, float* loss, float* row_loss,
+                     float* row_stats, void* stream);
+
+/* The gradient of grad_loss[0] * loss (grad_loss: one float on the device, NULL for 1):
+ *   grad[r, v] = grad_loss * scale * row_weight_r / T * (P q_v - sum of the p_j with index_j = v),
+ * P = sum_j p_j; a row that is left out gets zeros.  row_weight takes part as a factor, so a caller
+ * with a gradient for each row's loss passes it there.  grad: [rows, vocab] of type dtype, rows
+ * grad_stride apart; it may be `logits` itself (same stride). */
+int fdl_distill_topk_backward(const void* logits, int64_t logits_stride, int dtype, const void* teacher,
+                              int teacher_dtype, const int64_t* index, const float* teacher_lse,
+                              const float* row_weight, const float* row_stats, const float* grad_loss,
+                              int64_t rows, int64_t vocab, int64_t k, float temperature, float scale,
+                              void* grad, int64_t grad_stride, void* stream);
+
+/* Loss and gradient (for grad_loss = 1) in one call. */
+int fdl_distill_topk_with_grad(const void* logits, int64_t logits_stride, int dtype, const void* teacher,
+                               int teacher_dtype, const int64_t* index, const float* teacher_lse,
+                               const float* row_weight, int64_t rows, int64_t vocab, int64_t k,
+                               float temperature, float scale, float* loss, float* row_loss,
+                               float* row_stats, void* grad, int64_t grad_stride, void* stream);
+
+/* The norms after and before a block with its gate and the residual's scale, on row-major
+ * [rows, cols] tensors of type dtype:
+ *   u = norm_post(h) * post_gamma + post_beta
+ *   y = residual_scale * x + block_scale * act(gate) * u       (the new residual stream)
+ *   n = norm_pre(y) * pre_gamma + pre_beta                     (the next block's input)
+ * n is taken from y before y is rounded to its type.  gamma / beta: float [cols], NULL for 1 / 0.
+ * gate: [gate_rows, cols] of type dtype, gate_rows a divisor of rows, each gate row for
+ * rows / gate_rows consecutive rows (1: shared by all, rows: one for each); NULL with gate_rows 0.
+ * With post_kind FDL_NORM_NONE u is h itself (no post_gamma / post_beta); with pre_kind
+ * FDL_NORM_NONE there is no n (NULL).  stats (NULL, or [rows, 4] on the 16-byte grid) receives the
+ * rows' mean and 1 / sqrt(variance + eps) of h, then of y (0 and 1 for FDL_NORM_NONE, mean 0 for
+ * FDL_NORM_RMS).  y may be x and n may be h.  cols <= 32768. */
+int fdl_norm_residual(const void* x, const void* h, const void* gate, int64_t gate_rows, int gate_act,
+                      int post_kind, const float* post_gamma, const float* post_beta, int pre_kind,
+                      const float* pre_gamma, const float* pre_beta, void* y, void* n, float* stats,
+                      int64_t rows, int64_t cols, float residual_scale, float block_scale, float eps,
+                      int dtype, void* stream);
+
+/* Gradients of fdl_norm_residual from those of y and n (dy or dn may be NULL: none), with y, h and
+ * stats of the forward call.  Each of dx, dh, dgate (type dtype) and dpost_gamma, dpost_beta,
+ * dpre_gamma, dpre_beta (float [cols]) may be NULL: not wanted.  y may be NULL without dn.  dx may
+ * be dy, dh may be h or dn, and with one gate row for each row dgate may be gate.  Sums over rows are taken in a
+ * fixed order (no atomics).  scratch: fdl_norm_residual_backward_scratch_bytes, 256-byte aligned,
+ * need not be zeroed; calls that may overlap on the GPU must not share it. */
+size_t fdl_norm_residual_backward_scratch_bytes(int64_t rows, int64_t cols, int64_t gate_rows);
+int fdl_norm_residual_backward(const void* dy, const void* dn, const void* y, const void* h,
+                               const float* stats, const void* gate, int64_t gate_rows, int gate_act,
+                               int post_kind, const float* post_gamma, const float* post_beta,
+                               int pre_kind, const float* pre_gamma, void* dx, void* dh, void* dgate,
+                               float* dpost_gamma, float* dpost_beta, float* dpre_gamma,
+                               float* dpre_beta, int64_t rows, int64_t cols, float residual_scale,
+                               float block_scale, int dtype, void* scratch, size_t scratch_bytes,
+                               void* stream);
+
+/* Verification of drafted tokens: which of a sequence's drafted tokens stand, and the token after
+ * them, distributed as samples of the target model itself.  target: probabilities
+ * [batch, drafted + 1, vocab], draft: [batch, drafted, vocab] (NULL: the draft is certain of its
+ * tokens), of type dtype, the last dimension contiguous, the others with strides in elements (0 is
+ * allowed).  draft_tokens: [batch, drafted]; draft_len (NULL: drafted): how many of a sequence's
+ * there are; accept_u [batch, drafted] and sample_u [batch]: numbers in [0, 1).
+ *   Token i stands while accept_u_i * draft_i(token_i) < target_i(token_i) (product in float; a
+ *   token outside [0, vocab) falls).  The next token is drawn by sample_u from the weights
+ *   max(target_i - draft_i, 0) where token i fell, from target_len where all stand: the lowest v whose
+ *   running sum exceeds sample_u * total (64-bit sums; weights that are not positive finite numbers
+ *   count as 0; sample_u of 1 or NaN gives the last token with weight).  Without any weight the target's row
+ *   serves, and without any there the token is -1.
+ * tokens: [batch, drafted + 1], the standing tokens, the next one, then -1; accepted: [batch], how
+ * many stand.  drafted <= 65535, vocab < 2^30.  Deterministic; no scratch. */
+int fdl_verify_draft(const void* target, int64_t target_batch_stride, int64_t target_row_stride,
+                     const void* draft, int64_t draft_batch_stride, int64_t draft_row_stride,
+                     int dtype, const int64_t* draft_tokens, const int64_t* draft_len,
+                     const float* accept_u, const float* sample_u, int64_t batch, int64_t drafted,
+                     int64_t vocab, int64_t* tokens, int64_t* accepted, void* stream);
 
 /* ---- host-buffer entry points ---------------------------------------------------------- */
 
