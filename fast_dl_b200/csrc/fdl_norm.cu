@@ -61,6 +61,7 @@ struct NormParams {
     int cols;
     int post_kind, pre_kind, gate_act;
     float residual_scale, block_scale, eps;
+    unsigned int* error_flag;  // host-mapped; ring kernels
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -75,6 +76,11 @@ __device__ __forceinline__ uint32_t cluster_size() {
 }
 __device__ __forceinline__ void cluster_sync_all() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void store_remote(float* mine, uint32_t rank, float v) {
+    uint32_t remote;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_addr(mine)), "r"(rank));
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote), "f"(v) : "memory");
 }
 __device__ __forceinline__ void store_remote(float2* mine, uint32_t rank, float2 v) {
     uint32_t remote;
@@ -117,9 +123,17 @@ struct Team {
     }
 };
 
+// sigmoid and tanh from one exp2 and one reciprocal of the special-function unit (2^-22 each): with a gate
+// for each element they are a good part of a row's instructions.  tanh near 0, where 1 - 2 / (1 + e^2g)
+// would cancel, by its Taylor series (below 1/4 the next term is under 2^-26 of the sum).
 __device__ __forceinline__ float gate_value(int act, float g) {
-    if (act == FDL_GATE_SIGMOID) return 1.0f / (1.0f + expf(-g));
-    if (act == FDL_GATE_TANH) return tanhf(g);
+    if (act == FDL_GATE_SIGMOID) return __fdividef(1.0f, 1.0f + ex2_approx(-1.4426950408889634f * g));
+    if (act == FDL_GATE_TANH) {
+        const float far = 1.0f - __fdividef(2.0f, 1.0f + ex2_approx(2.8853900817779268f * g));
+        const float q = g * g;
+        const float near = g + g * q * (-1.0f / 3 + q * (2.0f / 15 + q * (-17.0f / 315 + q * (62.0f / 2835))));
+        return fabsf(g) < 0.25f ? near : far;
+    }
     return g;
 }
 // The slope of act at g, from a = act(g).
@@ -472,6 +486,533 @@ norm_residual_backward_kernel(const NormParams p) {
     if (!WARP && team.cluster > 1) cluster_sync_all();  // no CTA leaves while another may still write its sums
 }
 
+// ---- rows through shared memory ------------------------------------------------------------------
+//
+// For more rows than teams, on the 16-byte grid: one thread asks for whole row slices with bulk-async
+// copies, a few rows ahead of the row that the CTA works on, so the bytes in flight depend on neither
+// registers nor barriers.  gamma and beta (times the block's scale and a shared gate) lie in shared memory as
+// floats; a thread reads and writes only its own columns of them, so no barrier guards them.
+
+constexpr int kMaxStages = 4;
+
+struct RingPlan {
+    int stages;
+    int tiles;        // tensors a stage holds
+    int slice_packs;  // packs of a row that a CTA of the cluster owns
+};
+
+template <int NV>
+struct RingSums {
+    alignas(16) float buf[2][kMaxCluster * kMaxWarps * NV];
+};
+
+template <int NV>
+struct RingTeam {
+    RingSums<NV>* sums;
+    int phase, warps, cluster, rank;
+    // NV sums over the row's team: one barrier, alternating buffers.
+    __device__ __forceinline__ void sum(float (&v)[NV]) {
+        const int lane = threadIdx.x & (kWarp - 1), warp = threadIdx.x / kWarp;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) v[i] = warp_sum(v[i]);
+        float* at = sums->buf[phase];
+        phase ^= 1;
+        if (cluster == 1) {
+            if (lane == 0) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i) at[warp * NV + i] = v[i];
+            }
+            __syncthreads();
+        } else {
+            if (lane < cluster) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i) store_remote(&at[(rank * warps + warp) * NV + i], lane, v[i]);
+            }
+            cluster_sync_all();
+        }
+        const int n = warps * cluster;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) v[i] = 0.0f;
+        for (int w = 0; w < n; ++w) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) v[i] += at[w * NV + i];
+        }
+    }
+};
+
+// The consumer's side of the ring: waits, with a limit, for the copies of the stage that is next.
+struct RingWait {
+    uint64_t* full;
+    int stages, stage;
+    uint32_t parity;
+    bool failed;
+    __device__ __forceinline__ void wait(unsigned int* error_flag) {
+        if (!failed && !mbar_wait_bounded(&full[stage], parity)) {
+            failed = true;
+            atomicOr_system(error_flag, 1u);
+        }
+    }
+    __device__ __forceinline__ void next() {
+        if (++stage == stages) {
+            stage = 0;
+            parity ^= 1u;
+        }
+    }
+};
+
+template <int N>
+__device__ __forceinline__ void load_floats(const float* p, float (&v)[N]) {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+        const float4 f = reinterpret_cast<const float4*>(p)[i];
+        v[4 * i] = f.x; v[4 * i + 1] = f.y; v[4 * i + 2] = f.z; v[4 * i + 3] = f.w;
+    }
+}
+
+template <class T, int PACKS>
+__global__ void __launch_bounds__(512, PACKS * kPack<T> <= 8 ? 2 : 1)
+norm_residual_ring_kernel(const NormParams p, const RingPlan plan) {
+    constexpr int N = kPack<T>;
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ RingSums<1> sums;
+    __shared__ uint64_t full[kMaxStages];
+    RingTeam<1> team{&sums, 0, static_cast<int>(blockDim.x) / kWarp, static_cast<int>(cluster_size()),
+                     static_cast<int>(cluster_rank())};
+    const int t = threadIdx.x, threads = blockDim.x;
+    const int row_packs = p.cols / N;
+    const int first = team.rank * plan.slice_packs;
+    const int count = min(plan.slice_packs, row_packs - first);
+    const int tile_bytes = plan.slice_packs * 16;
+    const int64_t teams = gridDim.x / team.cluster, id = blockIdx.x / team.cluster;
+    // A contiguous run of rows a team: a shared gate changes seldom.
+    const int64_t from = p.rows * id / teams, to = p.rows * (id + 1) / teams;
+    const bool gate_each = p.gate != nullptr && p.rows_per_gate == 1;
+    float* const w1 = reinterpret_cast<float*>(smem + static_cast<size_t>(plan.stages) * plan.tiles * tile_bytes);
+    float* const w2 = w1 + plan.slice_packs * N;
+    float* const b1 = w2 + plan.slice_packs * N;
+    float* const b2 = p.post_beta != nullptr ? b1 + plan.slice_packs * N : b1;
+    if (t == 0) {
+        for (int s = 0; s < plan.stages; ++s) mbar_init(&full[s], 1);
+        fence_mbar_init();
+    }
+    if (team.cluster > 1) cluster_sync_all();  // every CTA has started before the first remote store
+    else __syncthreads();
+    pdl_wait();
+    auto request = [&](int64_t row, int stage) {
+        const size_t at = (static_cast<size_t>(row) * p.cols + static_cast<size_t>(first) * N) * sizeof(T);
+        unsigned char* to_smem = smem + static_cast<size_t>(stage) * plan.tiles * tile_bytes;
+        mbar_expect_tx(&full[stage], static_cast<uint32_t>(plan.tiles * count * 16));
+        bulk_g2s(to_smem, static_cast<const unsigned char*>(p.h) + at, count * 16, &full[stage]);
+        bulk_g2s(to_smem + tile_bytes, static_cast<const unsigned char*>(p.x) + at, count * 16, &full[stage]);
+        if (gate_each) bulk_g2s(to_smem + 2 * tile_bytes, static_cast<const unsigned char*>(p.gate) + at, count * 16, &full[stage]);
+    };
+    if (t == 0) {
+        for (int s = 0; s < plan.stages && from + s < to; ++s) request(from + s, s);
+    }
+#pragma unroll
+    for (int k = 0; k < PACKS; ++k) {
+        const int i = t + k * threads;
+        if (i >= count) continue;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const int c = (first + i) * N + e;
+            w1[i * N + e] = p.block_scale * (p.post_gamma != nullptr ? p.post_gamma[c] : 1.0f);
+            if (p.post_beta != nullptr) b1[i * N + e] = p.block_scale * p.post_beta[c];
+            w2[i * N + e] = p.pre_gamma != nullptr ? p.pre_gamma[c] : 1.0f;
+            if (p.pre_beta != nullptr) b2[i * N + e] = p.pre_beta[c];
+        }
+    }
+    RingWait ring{full, plan.stages, 0, 0, false};
+    const float inv = 1.0f / static_cast<float>(p.cols);
+    int64_t group = -1;
+    for (int64_t row = from; row < to; ++row) {
+        if (p.gate != nullptr && !gate_each && row / p.rows_per_gate != group) {  // another shared gate row: into w1, b1
+            group = row / p.rows_per_gate;
+#pragma unroll
+            for (int k = 0; k < PACKS; ++k) {
+                const int i = t + k * threads;
+                if (i >= count) continue;
+                float g[N];
+                Chunk<T, N>::load(static_cast<const T*>(p.gate) + group * p.cols + (first + i) * N, g);
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    const int c = (first + i) * N + e;
+                    const float a = p.block_scale * gate_value(p.gate_act, g[e]);
+                    w1[i * N + e] = a * (p.post_gamma != nullptr ? p.post_gamma[c] : 1.0f);
+                    if (p.post_beta != nullptr) b1[i * N + e] = a * p.post_beta[c];
+                }
+            }
+        }
+        ring.wait(p.error_flag);
+        const uint4* tile = reinterpret_cast<const uint4*>(smem + static_cast<size_t>(ring.stage) * plan.tiles * tile_bytes);
+        float v[PACKS][N];
+        uint4 xr[PACKS], gr[PACKS];
+#pragma unroll
+        for (int k = 0; k < PACKS; ++k) {
+            const int i = t + k * threads;
+            uint4 hr = make_uint4(0, 0, 0, 0);
+            xr[k] = gr[k] = hr;
+            if (i < count) {
+                hr = tile[i];
+                xr[k] = tile[plan.slice_packs + i];
+                if (gate_each) gr[k] = tile[2 * plan.slice_packs + i];
+            }
+            unpack(hr, v[k], T{});
+        }
+        bool released = false;
+        auto release = [&]() {  // behind a barrier that follows the reads above
+            if (!released && t == 0 && row + plan.stages < to && !ring.failed) request(row + plan.stages, ring.stage);
+            released = true;
+        };
+        auto moments = [&](int kind) {
+            if (kind == FDL_NORM_NONE) return make_float2(0.0f, 1.0f);
+            float mean = 0.0f;
+            if (kind == FDL_NORM_LAYER) {
+                float s[1] = {0.0f};
+#pragma unroll
+                for (int k = 0; k < PACKS; ++k) {
+#pragma unroll
+                    for (int e = 0; e < N; ++e) s[0] += v[k][e];
+                }
+                team.sum(s);
+                release();
+                mean = s[0] * inv;
+            }
+            float q[1] = {0.0f};
+#pragma unroll
+            for (int k = 0; k < PACKS; ++k) {
+                if (t + k * threads < count) {
+#pragma unroll
+                    for (int e = 0; e < N; ++e) q[0] += (v[k][e] - mean) * (v[k][e] - mean);
+                }
+            }
+            team.sum(q);
+            release();
+            return make_float2(mean, 1.0f / sqrtf(q[0] * inv + p.eps));
+        };
+        const float2 s1 = moments(p.post_kind);
+        const int64_t base = row * p.cols + static_cast<int64_t>(first) * N;
+#pragma unroll
+        for (int k = 0; k < PACKS; ++k) {
+            const int i = t + k * threads;
+            if (i >= count) continue;
+            float w[N], x[N];
+            load_floats(w1 + i * N, w);
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[k][e] = (v[k][e] - s1.x) * s1.y * w[e];
+            if (p.post_beta != nullptr) {
+                load_floats(b1 + i * N, w);
+#pragma unroll
+                for (int e = 0; e < N; ++e) v[k][e] += w[e];
+            }
+            if (gate_each) {
+                unpack(gr[k], w, T{});
+#pragma unroll
+                for (int e = 0; e < N; ++e) v[k][e] *= gate_value(p.gate_act, w[e]);
+            }
+            unpack(xr[k], x, T{});
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[k][e] += p.residual_scale * x[e];
+            Chunk<T, N>::store_stream(static_cast<T*>(p.y) + base + static_cast<int64_t>(i) * N, v[k]);
+        }
+        const float2 s2 = moments(p.pre_kind);
+        if (p.stats != nullptr && t == 0 && team.rank == 0) {
+            reinterpret_cast<float4*>(p.stats)[row] = make_float4(s1.x, s1.y, s2.x, s2.y);
+        }
+        if (p.n != nullptr) {
+#pragma unroll
+            for (int k = 0; k < PACKS; ++k) {
+                const int i = t + k * threads;
+                if (i >= count) continue;
+                float w[N];
+                load_floats(w2 + i * N, w);
+#pragma unroll
+                for (int e = 0; e < N; ++e) v[k][e] = (v[k][e] - s2.x) * s2.y * w[e];
+                if (p.pre_beta != nullptr) {
+                    load_floats(b2 + i * N, w);
+#pragma unroll
+                    for (int e = 0; e < N; ++e) v[k][e] += w[e];
+                }
+                Chunk<T, N>::store_stream(static_cast<T*>(p.n) + base + static_cast<int64_t>(i) * N, v[k]);
+            }
+        }
+        if (!released) {
+            __syncthreads();
+            release();
+        }
+        ring.next();
+    }
+    if (team.cluster > 1) cluster_sync_all();  // no CTA leaves while another may still write its sums
+}
+
+// BETA: sums for post_beta / pre_beta (and for a shared gate's share of post_beta) are kept.
+// Per task: s1 = sum D a hat(h), s0 = sum D a, with a = 1 where the gate is shared -- its factor, like the
+// block's scale, comes in when the task ends: dpost_gamma += scale a s1, dgate = scale act' (gamma s1 + beta s0).
+template <class T, int PACKS, bool BETA>
+__global__ void __launch_bounds__(512, 1)
+norm_residual_backward_ring_kernel(const NormParams p, const RingPlan plan) {
+    constexpr int N = kPack<T>;
+    constexpr int NB = BETA ? N : 1;
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ RingSums<2> sums;
+    __shared__ uint64_t full[kMaxStages];
+    RingTeam<2> team{&sums, 0, static_cast<int>(blockDim.x) / kWarp, static_cast<int>(cluster_size()),
+                     static_cast<int>(cluster_rank())};
+    const int t = threadIdx.x, threads = blockDim.x;
+    const int row_packs = p.cols / N;
+    const int first = team.rank * plan.slice_packs;
+    const int count = min(plan.slice_packs, row_packs - first);
+    const int tile_bytes = plan.slice_packs * 16;
+    const int64_t teams = gridDim.x / team.cluster, id = blockIdx.x / team.cluster;
+    const bool gate_each = p.gate != nullptr && p.rows_per_gate == 1;
+    const bool gate_shared = p.gate != nullptr && !gate_each;
+    float* const w1 = reinterpret_cast<float*>(smem + static_cast<size_t>(plan.stages) * plan.tiles * tile_bytes);
+    float* const w2 = w1 + plan.slice_packs * N;
+    // Places of the tensors in a stage; an absent one has none.
+    const int at_dn = 0, at_y = 1;
+    const int at_h = p.dn != nullptr ? 2 : 0;
+    const int at_dy = at_h + 1;
+    const int at_gate = at_dy + (p.dy != nullptr ? 1 : 0);
+    if (t == 0) {
+        for (int s = 0; s < plan.stages; ++s) mbar_init(&full[s], 1);
+        fence_mbar_init();
+    }
+    if (team.cluster > 1) cluster_sync_all();  // every CTA has started before the first remote store
+    else __syncthreads();
+    pdl_wait();
+    auto task_rows = [&](int64_t task, int64_t* begin, int64_t* end) {
+        const int64_t group = p.rows_per_gate == 1 ? 0 : task / p.tasks_per_gate;
+        const int64_t rows = p.rows_per_gate == 1 ? p.rows : p.rows_per_gate;
+        *begin = group * rows + (task - group * p.tasks_per_gate) * p.rows_per_task;
+        const int64_t stop = (group + 1) * rows;
+        *end = *begin + p.rows_per_task < stop ? *begin + p.rows_per_task : stop;
+    };
+    // The producer's own place in the same order of rows (thread 0).
+    int64_t ask_task = id, ask_row = 0, ask_end = 0;
+    if (ask_task < p.tasks) task_rows(ask_task, &ask_row, &ask_end);
+    auto request = [&](int stage) {
+        if (ask_task >= p.tasks) return;
+        const size_t at = (static_cast<size_t>(ask_row) * p.cols + static_cast<size_t>(first) * N) * sizeof(T);
+        unsigned char* to_smem = smem + static_cast<size_t>(stage) * plan.tiles * tile_bytes;
+        uint64_t* bar = &full[stage];
+        const uint32_t bytes = static_cast<uint32_t>(count) * 16u;
+        mbar_expect_tx(bar, static_cast<uint32_t>(plan.tiles) * bytes);
+        if (p.dn != nullptr) {
+            bulk_g2s(to_smem + at_dn * tile_bytes, static_cast<const unsigned char*>(p.dn) + at, bytes, bar);
+            bulk_g2s(to_smem + at_y * tile_bytes, static_cast<const unsigned char*>(p.y_in) + at, bytes, bar);
+        }
+        bulk_g2s(to_smem + at_h * tile_bytes, static_cast<const unsigned char*>(p.h) + at, bytes, bar);
+        if (p.dy != nullptr) bulk_g2s(to_smem + at_dy * tile_bytes, static_cast<const unsigned char*>(p.dy) + at, bytes, bar);
+        if (gate_each) bulk_g2s(to_smem + at_gate * tile_bytes, static_cast<const unsigned char*>(p.gate) + at, bytes, bar);
+        if (++ask_row == ask_end) {
+            ask_task += teams;
+            if (ask_task < p.tasks) task_rows(ask_task, &ask_row, &ask_end);
+        }
+    };
+    if (t == 0) {
+        for (int s = 0; s < plan.stages; ++s) request(s);
+    }
+    float s1[PACKS][N], s0[PACKS][NB], a2[PACKS][N], a3[PACKS][NB];
+#pragma unroll
+    for (int k = 0; k < PACKS; ++k) {
+        const int i = t + k * threads;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            s1[k][e] = a2[k][e] = 0.0f;
+            s0[k][e % NB] = a3[k][e % NB] = 0.0f;
+            if (i < count) {
+                const int c = (first + i) * N + e;
+                w1[i * N + e] = p.block_scale * (p.post_gamma != nullptr ? p.post_gamma[c] : 1.0f);
+                w2[i * N + e] = p.pre_gamma != nullptr ? p.pre_gamma[c] : 1.0f;
+            }
+        }
+    }
+    RingWait ring{full, plan.stages, 0, 0, false};
+    const float inv = 1.0f / static_cast<float>(p.cols);
+    bool flushed = false;  // the team's partial rows of post gamma / beta hold something
+    for (int64_t task = id; task < p.tasks; task += teams) {
+        int64_t from, to;
+        task_rows(task, &from, &to);
+        const int64_t group = task / p.tasks_per_gate;  // of a shared gate
+        if (gate_shared) {
+#pragma unroll
+            for (int k = 0; k < PACKS; ++k) {
+                const int i = t + k * threads;
+                if (i >= count) continue;
+                float g[N];
+                Chunk<T, N>::load(static_cast<const T*>(p.gate) + group * p.cols + (first + i) * N, g);
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    const int c = (first + i) * N + e;
+                    w1[i * N + e] = p.block_scale * gate_value(p.gate_act, g[e]) * (p.post_gamma != nullptr ? p.post_gamma[c] : 1.0f);
+                }
+            }
+        }
+        for (int64_t row = from; row < to; ++row) {
+            const float4 st = reinterpret_cast<const float4*>(p.stats_in)[row];
+            ring.wait(p.error_flag);
+            const uint4* tile = reinterpret_cast<const uint4*>(smem + static_cast<size_t>(ring.stage) * plan.tiles * tile_bytes);
+            const int64_t base = row * p.cols + static_cast<int64_t>(first) * N;
+            float d[PACKS][N], hat[PACKS][N];
+            float level = 0.0f, along = 0.0f;
+            if (p.dn != nullptr) {
+                float s[2] = {0.0f, 0.0f};
+                const float shift = -st.z * st.w;
+#pragma unroll
+                for (int k = 0; k < PACKS; ++k) {
+                    const int i = t + k * threads;
+                    if (i < count) {
+                        float w[N];
+                        unpack(tile[at_dn * plan.slice_packs + i], d[k], T{});
+                        unpack(tile[at_y * plan.slice_packs + i], hat[k], T{});
+                        load_floats(w2 + i * N, w);
+#pragma unroll
+                        for (int e = 0; e < N; ++e) {
+                            hat[k][e] = fmaf(hat[k][e], st.w, shift);
+                            a2[k][e] = fmaf(d[k][e], hat[k][e], a2[k][e]);
+                            if (BETA) a3[k][e % NB] += d[k][e];
+                            d[k][e] *= w[e];
+                            s[0] += d[k][e];
+                            s[1] = fmaf(d[k][e], hat[k][e], s[1]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < N; ++e) d[k][e] = hat[k][e] = 0.0f;
+                    }
+                }
+                team.sum(s);
+                level = p.pre_kind == FDL_NORM_LAYER ? s[0] * inv : 0.0f;
+                along = s[1] * inv;
+            } else {
+#pragma unroll
+                for (int k = 0; k < PACKS; ++k) {
+#pragma unroll
+                    for (int e = 0; e < N; ++e) d[k][e] = hat[k][e] = 0.0f;
+                }
+            }
+            float s[2] = {0.0f, 0.0f};
+            const float shift = -st.x * st.y;
+#pragma unroll
+            for (int k = 0; k < PACKS; ++k) {
+                const int i = t + k * threads;
+                if (i >= count) continue;
+                float w[N];
+                // D, and dx
+#pragma unroll
+                for (int e = 0; e < N; ++e) d[k][e] = st.w * (d[k][e] - level - hat[k][e] * along);
+                if (p.dy != nullptr) {
+                    unpack(tile[at_dy * plan.slice_packs + i], w, T{});
+#pragma unroll
+                    for (int e = 0; e < N; ++e) d[k][e] += w[e];
+                }
+                if (p.dx != nullptr) {
+#pragma unroll
+                    for (int e = 0; e < N; ++e) w[e] = p.residual_scale * d[k][e];
+                    Chunk<T, N>::store_stream(static_cast<T*>(p.dx) + base + static_cast<int64_t>(i) * N, w);
+                }
+                unpack(tile[at_h * plan.slice_packs + i], hat[k], T{});
+#pragma unroll
+                for (int e = 0; e < N; ++e) hat[k][e] = fmaf(hat[k][e], st.y, shift);
+                float scale[N];
+                load_floats(w1 + i * N, scale);  // block_scale * gamma (* a shared gate)
+                if (gate_each) {
+                    float a[N];
+                    unpack(tile[at_gate * plan.slice_packs + i], a, T{});
+#pragma unroll
+                    for (int e = 0; e < N; ++e) a[e] = gate_value(p.gate_act, a[e]);
+                    if (p.dgate != nullptr) {
+#pragma unroll
+                        for (int e = 0; e < N; ++e) {
+                            float u = hat[k][e] * scale[e];
+                            if (BETA && p.post_beta != nullptr) u += p.block_scale * p.post_beta[(first + i) * N + e];
+                            w[e] = d[k][e] * u * gate_slope(p.gate_act, a[e]);
+                        }
+                        Chunk<T, N>::store_stream(static_cast<T*>(p.dgate) + base + static_cast<int64_t>(i) * N, w);
+                    }
+#pragma unroll
+                    for (int e = 0; e < N; ++e) d[k][e] *= a[e];
+                }
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    s1[k][e] = fmaf(d[k][e], hat[k][e], s1[k][e]);
+                    if (BETA) s0[k][e % NB] += d[k][e];
+                    d[k][e] *= scale[e];
+                    s[0] += d[k][e];
+                    s[1] = fmaf(d[k][e], hat[k][e], s[1]);
+                }
+            }
+            if (p.post_kind != FDL_NORM_NONE) team.sum(s);
+            else __syncthreads();
+            if (t == 0 && !ring.failed) request(ring.stage);  // everybody has read the stage
+            if (p.dh != nullptr) {
+                level = p.post_kind == FDL_NORM_LAYER ? s[0] * inv : 0.0f;
+                along = p.post_kind != FDL_NORM_NONE ? s[1] * inv : 0.0f;
+#pragma unroll
+                for (int k = 0; k < PACKS; ++k) {
+                    const int i = t + k * threads;
+                    if (i >= count) continue;
+#pragma unroll
+                    for (int e = 0; e < N; ++e) d[k][e] = st.y * (d[k][e] - level - hat[k][e] * along);
+                    Chunk<T, N>::store_stream(static_cast<T*>(p.dh) + base + static_cast<int64_t>(i) * N, d[k]);
+                }
+            }
+            ring.next();
+        }
+        // The end of a task, or of the team's work: the sums under one shared gate.
+        const bool last = task + teams >= p.tasks;
+        if (!gate_shared && !last) continue;
+#pragma unroll
+        for (int k = 0; k < PACKS; ++k) {
+            const int i = t + k * threads;
+            if (i >= count) continue;
+            float g[N], a[N];
+            if (gate_shared) Chunk<T, N>::load(static_cast<const T*>(p.gate) + group * p.cols + (first + i) * N, g);
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const int c = (first + i) * N + e;
+                a[e] = gate_shared ? gate_value(p.gate_act, g[e]) : 1.0f;
+                const float b = BETA ? s0[k][e % NB] : 0.0f;
+                if (gate_shared && p.dgate != nullptr) {
+                    float u = (p.post_gamma != nullptr ? p.post_gamma[c] : 1.0f) * s1[k][e];
+                    if (BETA && p.post_beta != nullptr) u += p.post_beta[c] * b;
+                    g[e] = p.block_scale * gate_slope(p.gate_act, a[e]) * u;
+                }
+                float* const pg = p.partial[0] != nullptr ? p.partial[0] + id * p.cols + c : nullptr;
+                float* const pb = p.partial[1] != nullptr ? p.partial[1] + id * p.cols + c : nullptr;
+                if (pg != nullptr) *pg = (flushed ? *pg : 0.0f) + p.block_scale * a[e] * s1[k][e];
+                if (pb != nullptr) *pb = (flushed ? *pb : 0.0f) + p.block_scale * a[e] * b;
+                s1[k][e] = 0.0f;
+                if (BETA) s0[k][e % NB] = 0.0f;
+            }
+            if (gate_shared && p.dgate != nullptr) {
+                if (p.gate_partial != nullptr) {
+#pragma unroll
+                    for (int e = 0; e < N; ++e) p.gate_partial[task * p.cols + (first + i) * N + e] = g[e];
+                } else {
+                    Chunk<T, N>::store_stream(static_cast<T*>(p.dgate) + group * p.cols + (first + i) * N, g);
+                }
+            }
+        }
+        flushed = true;
+    }
+#pragma unroll
+    for (int k = 0; k < PACKS; ++k) {
+        const int i = t + k * threads;
+        if (i >= count) continue;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const int64_t c = id * p.cols + (first + i) * N + e;
+            if (p.partial[2] != nullptr) p.partial[2][c] = a2[k][e];
+            if (p.partial[3] != nullptr) p.partial[3][c] = BETA ? a3[k][e % NB] : 0.0f;
+            if (!flushed) {  // a team without a task
+                if (p.partial[0] != nullptr) p.partial[0][c] = 0.0f;
+                if (p.partial[1] != nullptr) p.partial[1][c] = 0.0f;
+            }
+        }
+    }
+    if (team.cluster > 1) cluster_sync_all();  // no CTA leaves while another may still write its sums
+}
+
 // out[g, c] = sum over r of part[g * each + r, c], rows in order; blockIdx.y picks one of the jobs.
 struct FoldJob {
     const float* part;
@@ -534,20 +1075,63 @@ Shape shape_of(int64_t cols) {
     return {false, threads, cluster, 1024 / threads < 1 ? 1 : 1024 / threads};
 }
 
+// The ring form: columns of a CTA, its threads and its stages; stages == 0: does not fit.
+struct RingShape {
+    int threads, cluster, blocks, per_thread;  // CTAs a row, CTAs an SM, columns a thread
+    RingPlan plan;
+    size_t smem;
+};
+
+// A thread owns 8 columns, or 16 of a 16-bit type: forward beyond 4096 columns, backward without sums for the
+// betas (their registers).  Stages take what is left of the shared memory of an SM, shared by as many CTAs as
+// 1024 threads make (backward: 512, with 128 registers each).
+RingShape ring_shape(int64_t cols, int dtype, int tiles, int weights, bool backward, bool beta) {
+    RingShape r = {};
+    const int n = 16 / static_cast<int>(dtype_bytes(dtype));
+    if (cols % n != 0 || cols <= kWarpCols) return r;  // no whole packs, or a warp a row
+    const int64_t packs = cols / n;
+    r.per_thread = dtype != FDL_F32 && (backward ? !beta : cols > 512 * 8) ? 16 : 8;
+    r.cluster = 1;
+    while (cols > static_cast<int64_t>(r.cluster) * 512 * r.per_thread) r.cluster *= 2;
+    r.plan.slice_packs = static_cast<int>(ceil_div(packs, r.cluster));
+    r.plan.tiles = tiles;
+    r.threads = static_cast<int>(ceil_div(ceil_div(r.plan.slice_packs, r.per_thread / n), kWarp)) * kWarp;
+    const int budget = backward || r.per_thread == 16 ? 512 : 1024;
+    r.blocks = budget / r.threads < 1 ? 1 : budget / r.threads > 16 ? 16 : budget / r.threads;
+    const size_t fixed = static_cast<size_t>(r.plan.slice_packs) * n * 4 * weights;
+    const size_t stage = static_cast<size_t>(r.plan.slice_packs) * 16 * tiles;
+    for (; r.blocks >= 1; --r.blocks) {  // fewer CTAs where less than two stages would fit
+        const size_t room = static_cast<size_t>(227 * 1024) / r.blocks - 4096;
+        if (room < fixed + 2 * stage) continue;
+        const size_t most = (room - fixed) / stage;
+        r.plan.stages = most > kMaxStages ? kMaxStages : static_cast<int>(most);
+        break;
+    }
+    if (r.blocks < 1) r.blocks = 1;
+    r.smem = fixed + stage * r.plan.stages;
+    return r;
+}
+
+// Backward: which form, and how the rows are dealt out.
 struct BackwardPlan {
-    Shape shape;
-    int64_t grid;   // CTAs
-    int64_t teams;  // partial rows of the sums over rows
+    bool ring;
+    Shape shape;      // direct form
+    RingShape rshape; // ring form
+    int64_t grid;     // CTAs
+    int64_t teams;    // partial rows of the sums over rows
     int64_t rows_per_gate, tasks_per_gate, rows_per_task, tasks;
 };
 
 // Tasks: every team gets about the same number of rows, and no task crosses a gate row's rows.
-BackwardPlan backward_plan(int64_t rows, int64_t cols, int64_t gate_rows, int sm_count) {
-    BackwardPlan b;
+BackwardPlan backward_plan(int64_t rows, int64_t cols, int64_t gate_rows, int sm_count, const RingShape* ring) {
+    BackwardPlan b = {};
     b.shape = shape_of(cols);
-    const int64_t per_cta = b.shape.warp ? b.shape.threads / kWarp : 1;
-    const int64_t slots = static_cast<int64_t>(sm_count) * b.shape.blocks / b.shape.cluster;  // teams of CTAs
-    const int64_t most = (slots < 1 ? 1 : slots) * per_cta;                                    // teams at once
+    b.ring = ring != nullptr;
+    if (ring != nullptr) b.rshape = *ring;
+    const int cluster = b.ring ? b.rshape.cluster : b.shape.cluster;
+    const int64_t per_cta = !b.ring && b.shape.warp ? b.shape.threads / kWarp : 1;
+    const int64_t slots = static_cast<int64_t>(sm_count) * (b.ring ? b.rshape.blocks : b.shape.blocks) / cluster;  // teams of CTAs
+    const int64_t most = (slots < 1 ? 1 : slots) * per_cta;                                                        // teams at once
     const bool gate_each = gate_rows == rows;
     const int64_t groups = gate_rows == 0 || gate_each ? 1 : gate_rows;
     const int64_t group = rows / groups;
@@ -569,8 +1153,8 @@ BackwardPlan backward_plan(int64_t rows, int64_t cols, int64_t gate_rows, int sm
     b.tasks_per_gate = ceil_div(group, b.rows_per_task);
     b.tasks = b.tasks_per_gate * groups;
     b.teams = b.tasks < most ? b.tasks : most;
-    b.grid = ceil_div(b.teams, per_cta) * b.shape.cluster;
-    b.teams = b.grid / b.shape.cluster * per_cta;
+    b.grid = ceil_div(b.teams, per_cta) * cluster;
+    b.teams = b.grid / cluster * per_cta;
     return b;
 }
 
@@ -623,6 +1207,38 @@ struct LaunchBackward {
     }
 };
 
+template <class K, class... Args>
+int launch_ring(K kernel, const NormParams& p, const RingShape& r, int64_t grid, cudaStream_t stream) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(r.smem));
+    if (e != cudaSuccess) return static_cast<int>(e);
+    return launch_ex(kernel, dim3(static_cast<unsigned int>(grid)), dim3(r.threads), r.smem, stream, dim3(r.cluster, 1, 1),
+                     tuning().pdl != 0, p, r.plan);
+}
+
+int launch_ring_forward(int dtype, const NormParams& p, const RingShape& r, int64_t grid, cudaStream_t stream) {
+    return with_dtype(dtype, [&](auto* tag) {
+        using T = std::remove_pointer_t<decltype(tag)>;
+        if constexpr (kPack<T> == 8) {
+            if (r.per_thread == 16) return launch_ring(norm_residual_ring_kernel<T, 2>, p, r, grid, stream);
+        }
+        return launch_ring(norm_residual_ring_kernel<T, 8 / kPack<T>>, p, r, grid, stream);
+    });
+}
+
+int launch_ring_backward(int dtype, bool beta, const NormParams& p, const RingShape& r, int64_t grid, cudaStream_t stream) {
+    return with_dtype(dtype, [&](auto* tag) {
+        using T = std::remove_pointer_t<decltype(tag)>;
+        if constexpr (kPack<T> == 8) {
+            if (r.per_thread == 16) {
+                return beta ? launch_ring(norm_residual_backward_ring_kernel<T, 2, true>, p, r, grid, stream)
+                            : launch_ring(norm_residual_backward_ring_kernel<T, 2, false>, p, r, grid, stream);
+            }
+        }
+        return beta ? launch_ring(norm_residual_backward_ring_kernel<T, 8 / kPack<T>, true>, p, r, grid, stream)
+                    : launch_ring(norm_residual_backward_ring_kernel<T, 8 / kPack<T>, false>, p, r, grid, stream);
+    });
+}
+
 }  // namespace
 
 }  // namespace fdl
@@ -656,22 +1272,48 @@ int fdl_norm_residual(const void* x, const void* h, const void* gate, int64_t ga
     p.cols = static_cast<int>(cols);
     p.post_kind = post_kind; p.pre_kind = pre_kind; p.gate_act = gate_act;
     p.residual_scale = residual_scale; p.block_scale = block_scale; p.eps = eps;
+    const bool vec = packs_fit(dtype, cols, {x, h, gate, y, n});
     const Shape s = shape_of(cols);
+    if (vec) {
+        const int weights = 2 + (post_beta != nullptr) + (pre_beta != nullptr);
+        const RingShape r = ring_shape(cols, dtype, 2 + (gate != nullptr && gate_rows == rows), weights, false, false);
+        const int64_t teams = r.plan.stages >= 2 ? static_cast<int64_t>(info->sm_count) * r.blocks / r.cluster : rows;
+        if (rows > teams) {
+            status = error_flag_device_ptr(&p.error_flag);
+            if (status != FDL_OK) return status;
+            return launch_ring_forward(dtype, p, r, teams * r.cluster, as_stream(stream));
+        }
+    }
     const int64_t per_cta = s.warp ? s.threads / kWarp : 1;
     const int64_t slots = static_cast<int64_t>(info->sm_count) * s.blocks / s.cluster;
     const int64_t work = ceil_div(rows, per_cta);
     const int64_t grid = (work < slots ? work : slots < 1 ? 1 : slots) * s.cluster;
-    return dispatch<LaunchForward>(dtype, packs_fit(dtype, cols, {x, h, gate, y, n}), s.warp, p, s, grid, as_stream(stream));
+    return dispatch<LaunchForward>(dtype, vec, s.warp, p, s, grid, as_stream(stream));
 }
 
+// Room for whichever form the call takes: the direct form, or the ring form with any of its tiles and types.
 size_t fdl_norm_residual_backward_scratch_bytes(int64_t rows, int64_t cols, int64_t gate_rows) {
     if (rows <= 0 || cols <= 0 || cols > kMaxCols || gate_rows < 0) return 0;
     if (gate_rows > 0 && (gate_rows > rows || rows % gate_rows != 0)) return 0;
     int status = FDL_OK;
     const DeviceInfo* info = current_device_info(&status);
-    const BackwardPlan b = backward_plan(rows, cols, gate_rows, info == nullptr ? 148 : info->sm_count);
-    const int64_t gate_part = gate_rows == 0 || gate_rows == rows || b.tasks_per_gate == 1 ? 0 : b.tasks;
-    const int64_t floats = (4 * b.teams + gate_part) * cols;
+    const int sms = info == nullptr ? 148 : info->sm_count;
+    int64_t floats = 0;
+    auto add = [&](const RingShape* r) {
+        const BackwardPlan b = backward_plan(rows, cols, gate_rows, sms, r);
+        const int64_t gate_part = gate_rows == 0 || gate_rows == rows || b.tasks_per_gate == 1 ? 0 : b.tasks;
+        const int64_t f = (4 * b.teams + gate_part) * cols;
+        if (f > floats) floats = f;
+    };
+    add(nullptr);
+    for (int dtype : {static_cast<int>(FDL_F32), static_cast<int>(FDL_BF16)}) {
+        for (int tiles = 2; tiles <= 5; ++tiles) {
+            for (int few = 0; few < 2; ++few) {
+                const RingShape r = ring_shape(cols, dtype, tiles, 2, true, few == 0);
+                if (r.plan.stages >= 2) add(&r);
+            }
+        }
+    }
     return static_cast<size_t>(ceil_div(floats * 4, 256) * 256);
 }
 
@@ -713,7 +1355,12 @@ int fdl_norm_residual_backward(const void* dy, const void* dn, const void* y, co
     }
     const DeviceInfo* info = current_device_info(&status);
     if (info == nullptr) return status;
-    const BackwardPlan b = backward_plan(rows, cols, gate_rows, info->sm_count);
+    const bool vec = packs_fit(dtype, cols, {dy, dn, y, h, gate, dx, dh, dgate});
+    const bool beta = dpost_beta != nullptr || dpre_beta != nullptr || (post_beta != nullptr && dgate != nullptr);
+    const int tiles = 1 + (dn != nullptr ? 2 : 0) + (dy != nullptr) + (gate != nullptr && gate_rows == rows);
+    const RingShape r = ring_shape(cols, dtype, tiles, 2, true, beta);
+    const bool ring = vec && r.plan.stages >= 2;
+    const BackwardPlan b = backward_plan(rows, cols, gate_rows, info->sm_count, ring ? &r : nullptr);
     NormParams p = {};
     p.dy = dy; p.dn = dn; p.y_in = y; p.h = h; p.stats_in = stats; p.gate = gate;
     p.post_gamma = post_gamma; p.post_beta = post_beta; p.pre_gamma = pre_gamma;
@@ -742,8 +1389,12 @@ int fdl_norm_residual_backward(const void* dy, const void* dn, const void* y, co
         jobs.job[njobs++] = {at, dgate, dtype, gate_rows, b.tasks_per_gate};
         groups = gate_rows;
     }
-    status = dispatch<LaunchBackward>(dtype, packs_fit(dtype, cols, {dy, dn, y, h, gate, dx, dh, dgate}), b.shape.warp, p,
-                                      b.shape, b.grid, s);
+    if (ring) {
+        status = error_flag_device_ptr(&p.error_flag);
+        if (status == FDL_OK) status = launch_ring_backward(dtype, beta, p, r, b.grid, s);
+    } else {
+        status = dispatch<LaunchBackward>(dtype, vec, b.shape.warp, p, b.shape, b.grid, s);
+    }
     if (status != FDL_OK || njobs == 0) return status;
     const dim3 grid(static_cast<unsigned int>(ceil_div(cols, kFoldX)), static_cast<unsigned int>(njobs),
                     static_cast<unsigned int>(groups < 64 ? groups : 64));

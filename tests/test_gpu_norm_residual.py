@@ -249,6 +249,19 @@ def test_many_rows_and_their_gates(fdl, cuda, rows, gates, cols):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,cols,gates", [(1400, 264, 7), (2500, 512, 1), (601, 1000, 601), (700, 2048, 0), (450, 4096, 450),
+                                             (450, 4096, 150), (330, 4104, 3), (400, 8192, 2), (151, 8200, 1), (160, 16384, 160),
+                                             (90, 32768, 9)])
+def test_more_rows_than_teams(fdl, cuda, rows, cols, gates, kind):
+    """Whole packs a row, and several rows for each team, from one to eight CTAs wide."""
+    check(fdl, Case(rows, cols, kind, RMS, RMS, gates, SIGMOID if gates else PLAIN).cuda(), ("both", "dn"))
+    check(fdl, Case(rows, cols, kind, LAYER, LAYER, gates, TANH if gates else PLAIN, seed=2).cuda(), ("both", "dy"))
+    check(fdl, Case(rows, cols, kind, NONE, NONE, gates, PLAIN).cuda())
+    fdl.take_device_error()
+
+
+@pytest.mark.gpu
 def test_shifted_starts_take_the_element_path(fdl, cuda):
     c = Case(5, 512, "bf16", LAYER, LAYER, 5, TANH).cuda()
     y, n, stats = c.forward(fdl)
@@ -317,16 +330,22 @@ def test_offsets_beyond_32_bits(fdl, cuda):
     x = torch.zeros(rows, cols, dtype=torch.bfloat16, device="cuda")
     h = torch.zeros(rows, cols, dtype=torch.bfloat16, device="cuda")
     x[-4:], h[-4:] = c.x, c.h
-    y, n, stats = c.forward(fdl)
     yy, nn, ss = fdl.norm_residual(x, h, eps=c.eps, **c.common())
-    assert torch.equal(yy[-4:], y) and torch.equal(nn[-4:], n) and torch.equal(ss[-4:], stats)
+    want_y, want_n, tol_y, tol_n, want_stats = c.want_forward()
+    close(yy[-4:], want_y, tol_y, "y")
+    close(nn[-4:], want_n, tol_n, "n")
     assert not yy[:-4].any() and not nn[:-4].any()
     dy = torch.zeros_like(x)
     dy[-4:] = c.dy
     del x, nn
-    want = c.backward(fdl, y, stats, c.dy, None)
     got = fdl.norm_residual_backward(dy, None, yy, h, ss, **c.common())
-    assert torch.equal(got["x"][-4:], want["x"]) and torch.equal(got["h"][-4:], want["h"])
+    want, tol = c.want_backward(yy[-4:], ss[-4:], c.dy, None)
+    for name in ("x", "h"):
+        close(got[name][-4:], want[name], tol[name], name)
+        assert not got[name][:-4].any()
+    c.rows = rows  # the sums run over all rows
+    want, tol = c.want_backward(yy[-4:], ss[-4:], c.dy, None)
+    close(got["post_gamma"], want["post_gamma"], tol["post_gamma"], "post_gamma")
 
 
 @pytest.mark.gpu
