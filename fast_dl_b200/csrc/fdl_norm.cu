@@ -123,24 +123,39 @@ struct Team {
     }
 };
 
-// sigmoid and tanh from one exp2 and one reciprocal of the special-function unit (2^-22 each): with a gate
-// for each element they are a good part of a row's instructions.  tanh near 0, where 1 - 2 / (1 + e^2g)
+// sigmoid and tanh from one exp2 and one reciprocal of the special-function unit (2^-22 and 2^-23): with a
+// gate for each element they are a good part of a row's instructions.  tanh near 0, where 1 - 2 / (1 + e^2g)
 // would cancel, by its Taylor series (below 1/4 the next term is under 2^-26 of the sum).
-__device__ __forceinline__ float gate_value(int act, float g) {
-    if (act == FDL_GATE_SIGMOID) return __fdividef(1.0f, 1.0f + ex2_approx(-1.4426950408889634f * g));
-    if (act == FDL_GATE_TANH) {
-        const float far = 1.0f - __fdividef(2.0f, 1.0f + ex2_approx(2.8853900817779268f * g));
-        const float q = g * g;
-        const float near = g + g * q * (-1.0f / 3 + q * (2.0f / 15 + q * (-17.0f / 315 + q * (62.0f / 2835))));
-        return fabsf(g) < 0.25f ? near : far;
-    }
-    return g;
+__device__ __forceinline__ float rcp_approx(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
-// The slope of act at g, from a = act(g).
-__device__ __forceinline__ float gate_slope(int act, float a) {
-    if (act == FDL_GATE_SIGMOID) return a * (1.0f - a);
-    if (act == FDL_GATE_TANH) return 1.0f - a * a;
-    return 1.0f;
+template <int N>
+__device__ __forceinline__ void gate_values(int act, float (&g)[N]) {  // one branch for the N of them
+    if (act == FDL_GATE_SIGMOID) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) g[e] = rcp_approx(1.0f + ex2_approx(-1.4426950408889634f * g[e]));
+    } else if (act == FDL_GATE_TANH) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const float far = 1.0f - 2.0f * rcp_approx(1.0f + ex2_approx(2.8853900817779268f * g[e]));
+            const float q = g[e] * g[e];
+            const float near = g[e] + g[e] * q * (-1.0f / 3 + q * (2.0f / 15 + q * (-17.0f / 315 + q * (62.0f / 2835))));
+            g[e] = fabsf(g[e]) < 0.25f ? near : far;
+        }
+    }
+}
+// v *= the slope of act, from a = act(g).
+template <int N>
+__device__ __forceinline__ void times_slope(int act, const float (&a)[N], float (&v)[N]) {
+    if (act == FDL_GATE_SIGMOID) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] *= a[e] - a[e] * a[e];
+    } else if (act == FDL_GATE_TANH) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] *= 1.0f - a[e] * a[e];
+    }
 }
 
 template <int N, int PACKS>
@@ -253,8 +268,9 @@ norm_residual_kernel(const NormParams p) {
             load_row<T>(static_cast<const T*>(p.gate) + row / p.rows_per_gate * p.cols, own, p.cols, w);
 #pragma unroll
             for (int k = 0; k < PACKS; ++k) {
+                gate_values(p.gate_act, w[k]);
 #pragma unroll
-                for (int e = 0; e < N; ++e) h[k][e] *= gate_value(p.gate_act, w[k][e]);
+                for (int e = 0; e < N; ++e) h[k][e] *= w[k][e];
             }
         }
 #pragma unroll
@@ -335,10 +351,7 @@ norm_residual_backward_kernel(const NormParams p) {
         if (p.gate != nullptr && !gate_each) {
             load_row<T>(static_cast<const T*>(p.gate) + group * p.cols, own, p.cols, gate);
 #pragma unroll
-            for (int k = 0; k < PACKS; ++k) {
-#pragma unroll
-                for (int e = 0; e < N; ++e) gate[k][e] = gate_value(p.gate_act, gate[k][e]);
-            }
+            for (int k = 0; k < PACKS; ++k) gate_values(p.gate_act, gate[k]);
         }
         for (int64_t row = from; row < to; ++row) {
             const int64_t base = row * p.cols;
@@ -388,10 +401,7 @@ norm_residual_backward_kernel(const NormParams p) {
             if (p.gate != nullptr && gate_each) {
                 load_row<T>(static_cast<const T*>(p.gate) + base, own, p.cols, gate);
 #pragma unroll
-                for (int k = 0; k < PACKS; ++k) {
-#pragma unroll
-                    for (int e = 0; e < N; ++e) gate[k][e] = gate_value(p.gate_act, gate[k][e]);
-                }
+                for (int k = 0; k < PACKS; ++k) gate_values(p.gate_act, gate[k]);
             }
             if (p.dx != nullptr) {
 #pragma unroll
@@ -418,9 +428,9 @@ norm_residual_backward_kernel(const NormParams p) {
 #pragma unroll
                     for (int e = 0; e < N; ++e) {
                         u[k][e] = d[k][e] * (hat[k][e] * u[k][e] + w[k][e]);
-                        if (gate_each) u[k][e] *= gate_slope(p.gate_act, gate[k][e]);
-                        else gsum[k][e] += u[k][e];
+                        gsum[k][e] += u[k][e];
                     }
+                    if (gate_each) times_slope(p.gate_act, gate[k], u[k]);
                     if (gate_each && own.col(k) < p.cols) {
                         Chunk<T, N>::store_stream(static_cast<T*>(p.dgate) + base + own.col(k), u[k]);
                     }
@@ -462,8 +472,7 @@ norm_residual_backward_kernel(const NormParams p) {
 #pragma unroll
             for (int k = 0; k < PACKS; ++k) {
                 if (own.col(k) >= p.cols) continue;
-#pragma unroll
-                for (int e = 0; e < N; ++e) gsum[k][e] *= gate_slope(p.gate_act, gate[k][e]);
+                times_slope(p.gate_act, gate[k], gsum[k]);
                 if (p.gate_partial != nullptr) {
 #pragma unroll
                     for (int e = 0; e < N; ++e) p.gate_partial[task * p.cols + own.col(k) + e] = gsum[k][e];
@@ -530,13 +539,16 @@ struct RingTeam {
             }
             cluster_sync_all();
         }
+        // Each warp folds the partial sums by itself, all in the same order.
         const int n = warps * cluster;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) v[i] = 0.0f;
-        for (int w = 0; w < n; ++w) {
+        for (int i = 0; i < NV; ++i) v[i] = lane < n ? at[lane * NV + i] : 0.0f;
+        for (int w = lane + kWarp; w < n; w += kWarp) {
 #pragma unroll
             for (int i = 0; i < NV; ++i) v[i] += at[w * NV + i];
         }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) v[i] = warp_sum(v[i]);
     }
 };
 
@@ -560,17 +572,30 @@ struct RingWait {
     }
 };
 
+// The floats of pack i, kept as N / 4 arrays of 128-bit groups so that lanes next to each other read next
+// to each other.
 template <int N>
-__device__ __forceinline__ void load_floats(const float* p, float (&v)[N]) {
+__device__ __forceinline__ void load_floats(const float4* w, int i, int packs, float (&v)[N]) {
 #pragma unroll
-    for (int i = 0; i < N / 4; ++i) {
-        const float4 f = reinterpret_cast<const float4*>(p)[i];
-        v[4 * i] = f.x; v[4 * i + 1] = f.y; v[4 * i + 2] = f.z; v[4 * i + 3] = f.w;
+    for (int q = 0; q < N / 4; ++q) {
+        const float4 f = w[q * packs + i];
+        v[4 * q] = f.x; v[4 * q + 1] = f.y; v[4 * q + 2] = f.z; v[4 * q + 3] = f.w;
     }
+}
+template <int N>
+__device__ __forceinline__ void keep_floats(float4* w, int i, int packs, const float (&v)[N]) {
+#pragma unroll
+    for (int q = 0; q < N / 4; ++q) w[q * packs + i] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+}
+// scale * w[col ...], or scale where there is no w.
+template <int N>
+__device__ __forceinline__ void fetch_floats(const float* w, int col, float scale, float (&v)[N]) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] = w != nullptr ? scale * w[col + e] : scale;
 }
 
 template <class T, int PACKS>
-__global__ void __launch_bounds__(512, PACKS * kPack<T> <= 8 ? 2 : 1)
+__global__ void __launch_bounds__(512, 2)
 norm_residual_ring_kernel(const NormParams p, const RingPlan plan) {
     constexpr int N = kPack<T>;
     extern __shared__ __align__(128) unsigned char smem[];
@@ -579,18 +604,18 @@ norm_residual_ring_kernel(const NormParams p, const RingPlan plan) {
     RingTeam<1> team{&sums, 0, static_cast<int>(blockDim.x) / kWarp, static_cast<int>(cluster_size()),
                      static_cast<int>(cluster_rank())};
     const int t = threadIdx.x, threads = blockDim.x;
-    const int row_packs = p.cols / N;
-    const int first = team.rank * plan.slice_packs;
-    const int count = min(plan.slice_packs, row_packs - first);
-    const int tile_bytes = plan.slice_packs * 16;
+    const int row_packs = p.cols / N, slice = plan.slice_packs;
+    const int first = team.rank * slice;
+    const int count = min(slice, row_packs - first);
     const int64_t teams = gridDim.x / team.cluster, id = blockIdx.x / team.cluster;
     // A contiguous run of rows a team: a shared gate changes seldom.
     const int64_t from = p.rows * id / teams, to = p.rows * (id + 1) / teams;
     const bool gate_each = p.gate != nullptr && p.rows_per_gate == 1;
-    float* const w1 = reinterpret_cast<float*>(smem + static_cast<size_t>(plan.stages) * plan.tiles * tile_bytes);
-    float* const w2 = w1 + plan.slice_packs * N;
-    float* const b1 = w2 + plan.slice_packs * N;
-    float* const b2 = p.post_beta != nullptr ? b1 + plan.slice_packs * N : b1;
+    uint4* const stages = reinterpret_cast<uint4*>(smem);  // [stages][tiles][slice]
+    float4* const w1 = reinterpret_cast<float4*>(stages + static_cast<size_t>(plan.stages) * plan.tiles * slice);
+    float4* const w2 = w1 + slice * (N / 4);
+    float4* const b1 = w2 + slice * (N / 4);
+    float4* const b2 = p.post_beta != nullptr ? b1 + slice * (N / 4) : b1;
     if (t == 0) {
         for (int s = 0; s < plan.stages; ++s) mbar_init(&full[s], 1);
         fence_mbar_init();
@@ -600,33 +625,48 @@ norm_residual_ring_kernel(const NormParams p, const RingPlan plan) {
     pdl_wait();
     auto request = [&](int64_t row, int stage) {
         const size_t at = (static_cast<size_t>(row) * p.cols + static_cast<size_t>(first) * N) * sizeof(T);
-        unsigned char* to_smem = smem + static_cast<size_t>(stage) * plan.tiles * tile_bytes;
+        uint4* tile = stages + static_cast<size_t>(stage) * plan.tiles * slice;
         mbar_expect_tx(&full[stage], static_cast<uint32_t>(plan.tiles * count * 16));
-        bulk_g2s(to_smem, static_cast<const unsigned char*>(p.h) + at, count * 16, &full[stage]);
-        bulk_g2s(to_smem + tile_bytes, static_cast<const unsigned char*>(p.x) + at, count * 16, &full[stage]);
-        if (gate_each) bulk_g2s(to_smem + 2 * tile_bytes, static_cast<const unsigned char*>(p.gate) + at, count * 16, &full[stage]);
+        bulk_g2s(tile, static_cast<const unsigned char*>(p.h) + at, count * 16, &full[stage]);
+        bulk_g2s(tile + slice, static_cast<const unsigned char*>(p.x) + at, count * 16, &full[stage]);
+        if (gate_each) bulk_g2s(tile + 2 * slice, static_cast<const unsigned char*>(p.gate) + at, count * 16, &full[stage]);
     };
     if (t == 0) {
         for (int s = 0; s < plan.stages && from + s < to; ++s) request(from + s, s);
     }
+    auto weigh = [&](float (&scale)[N], int i) {  // post_gamma, post_beta times the block's scale (and a shared gate)
+        float w[N];
+        fetch_floats(p.post_gamma, (first + i) * N, 1.0f, w);
+#pragma unroll
+        for (int e = 0; e < N; ++e) w[e] *= scale[e];
+        keep_floats(w1, i, slice, w);
+        if (p.post_beta != nullptr) {
+            fetch_floats(p.post_beta, (first + i) * N, 1.0f, w);
+#pragma unroll
+            for (int e = 0; e < N; ++e) w[e] *= scale[e];
+            keep_floats(b1, i, slice, w);
+        }
+    };
 #pragma unroll
     for (int k = 0; k < PACKS; ++k) {
         const int i = t + k * threads;
         if (i >= count) continue;
+        float w[N];
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-            const int c = (first + i) * N + e;
-            w1[i * N + e] = p.block_scale * (p.post_gamma != nullptr ? p.post_gamma[c] : 1.0f);
-            if (p.post_beta != nullptr) b1[i * N + e] = p.block_scale * p.post_beta[c];
-            w2[i * N + e] = p.pre_gamma != nullptr ? p.pre_gamma[c] : 1.0f;
-            if (p.pre_beta != nullptr) b2[i * N + e] = p.pre_beta[c];
+        for (int e = 0; e < N; ++e) w[e] = p.block_scale;
+        weigh(w, i);
+        fetch_floats(p.pre_gamma, (first + i) * N, 1.0f, w);
+        keep_floats(w2, i, slice, w);
+        if (p.pre_beta != nullptr) {
+            fetch_floats(p.pre_beta, (first + i) * N, 1.0f, w);
+            keep_floats(b2, i, slice, w);
         }
     }
     RingWait ring{full, plan.stages, 0, 0, false};
     const float inv = 1.0f / static_cast<float>(p.cols);
     int64_t group = -1;
     for (int64_t row = from; row < to; ++row) {
-        if (p.gate != nullptr && !gate_each && row / p.rows_per_gate != group) {  // another shared gate row: into w1, b1
+        if (p.gate != nullptr && !gate_each && row / p.rows_per_gate != group) {  // another shared gate row
             group = row / p.rows_per_gate;
 #pragma unroll
             for (int k = 0; k < PACKS; ++k) {
@@ -634,36 +674,20 @@ norm_residual_ring_kernel(const NormParams p, const RingPlan plan) {
                 if (i >= count) continue;
                 float g[N];
                 Chunk<T, N>::load(static_cast<const T*>(p.gate) + group * p.cols + (first + i) * N, g);
+                gate_values(p.gate_act, g);
 #pragma unroll
-                for (int e = 0; e < N; ++e) {
-                    const int c = (first + i) * N + e;
-                    const float a = p.block_scale * gate_value(p.gate_act, g[e]);
-                    w1[i * N + e] = a * (p.post_gamma != nullptr ? p.post_gamma[c] : 1.0f);
-                    if (p.post_beta != nullptr) b1[i * N + e] = a * p.post_beta[c];
-                }
+                for (int e = 0; e < N; ++e) g[e] *= p.block_scale;
+                weigh(g, i);
             }
         }
         ring.wait(p.error_flag);
-        const uint4* tile = reinterpret_cast<const uint4*>(smem + static_cast<size_t>(ring.stage) * plan.tiles * tile_bytes);
+        const uint4* tile = stages + static_cast<size_t>(ring.stage) * plan.tiles * slice;
         float v[PACKS][N];
-        uint4 xr[PACKS], gr[PACKS];
 #pragma unroll
         for (int k = 0; k < PACKS; ++k) {
             const int i = t + k * threads;
-            uint4 hr = make_uint4(0, 0, 0, 0);
-            xr[k] = gr[k] = hr;
-            if (i < count) {
-                hr = tile[i];
-                xr[k] = tile[plan.slice_packs + i];
-                if (gate_each) gr[k] = tile[2 * plan.slice_packs + i];
-            }
-            unpack(hr, v[k], T{});
+            unpack(i < count ? tile[i] : make_uint4(0, 0, 0, 0), v[k], T{});
         }
-        bool released = false;
-        auto release = [&]() {  // behind a barrier that follows the reads above
-            if (!released && t == 0 && row + plan.stages < to && !ring.failed) request(row + plan.stages, ring.stage);
-            released = true;
-        };
         auto moments = [&](int kind) {
             if (kind == FDL_NORM_NONE) return make_float2(0.0f, 1.0f);
             float mean = 0.0f;
@@ -675,7 +699,6 @@ norm_residual_ring_kernel(const NormParams p, const RingPlan plan) {
                     for (int e = 0; e < N; ++e) s[0] += v[k][e];
                 }
                 team.sum(s);
-                release();
                 mean = s[0] * inv;
             }
             float q[1] = {0.0f};
@@ -683,62 +706,69 @@ norm_residual_ring_kernel(const NormParams p, const RingPlan plan) {
             for (int k = 0; k < PACKS; ++k) {
                 if (t + k * threads < count) {
 #pragma unroll
-                    for (int e = 0; e < N; ++e) q[0] += (v[k][e] - mean) * (v[k][e] - mean);
+                    for (int e = 0; e < N; ++e) q[0] = fmaf(v[k][e] - mean, v[k][e] - mean, q[0]);
                 }
             }
             team.sum(q);
-            release();
-            return make_float2(mean, 1.0f / sqrtf(q[0] * inv + p.eps));
+            return make_float2(mean, 1.0f / sqrtf(fmaf(q[0], inv, p.eps)));
         };
         const float2 s1 = moments(p.post_kind);
         const int64_t base = row * p.cols + static_cast<int64_t>(first) * N;
+        const float shift1 = -s1.x * s1.y;
 #pragma unroll
         for (int k = 0; k < PACKS; ++k) {
             const int i = t + k * threads;
             if (i >= count) continue;
-            float w[N], x[N];
-            load_floats(w1 + i * N, w);
-#pragma unroll
-            for (int e = 0; e < N; ++e) v[k][e] = (v[k][e] - s1.x) * s1.y * w[e];
+            float w[N];
+            load_floats(w1, i, slice, w);
             if (p.post_beta != nullptr) {
-                load_floats(b1 + i * N, w);
+                float b[N];
+                load_floats(b1, i, slice, b);
 #pragma unroll
-                for (int e = 0; e < N; ++e) v[k][e] += w[e];
+                for (int e = 0; e < N; ++e) v[k][e] = fmaf(fmaf(v[k][e], s1.y, shift1), w[e], b[e]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < N; ++e) v[k][e] = fmaf(v[k][e], s1.y, shift1) * w[e];
             }
+            float x[N];
+            unpack(tile[slice + i], x, T{});
             if (gate_each) {
-                unpack(gr[k], w, T{});
+                unpack(tile[2 * slice + i], w, T{});
+                gate_values(p.gate_act, w);
 #pragma unroll
-                for (int e = 0; e < N; ++e) v[k][e] *= gate_value(p.gate_act, w[e]);
+                for (int e = 0; e < N; ++e) v[k][e] = fmaf(v[k][e], w[e], p.residual_scale * x[e]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < N; ++e) v[k][e] = fmaf(p.residual_scale, x[e], v[k][e]);
             }
-            unpack(xr[k], x, T{});
-#pragma unroll
-            for (int e = 0; e < N; ++e) v[k][e] += p.residual_scale * x[e];
             Chunk<T, N>::store_stream(static_cast<T*>(p.y) + base + static_cast<int64_t>(i) * N, v[k]);
         }
         const float2 s2 = moments(p.pre_kind);
+        if (p.pre_kind == FDL_NORM_NONE) __syncthreads();
+        // Behind a barrier that follows everybody's reads of the stage.
+        if (t == 0 && row + plan.stages < to && !ring.failed) request(row + plan.stages, ring.stage);
         if (p.stats != nullptr && t == 0 && team.rank == 0) {
             reinterpret_cast<float4*>(p.stats)[row] = make_float4(s1.x, s1.y, s2.x, s2.y);
         }
         if (p.n != nullptr) {
+            const float shift2 = -s2.x * s2.y;
 #pragma unroll
             for (int k = 0; k < PACKS; ++k) {
                 const int i = t + k * threads;
                 if (i >= count) continue;
                 float w[N];
-                load_floats(w2 + i * N, w);
-#pragma unroll
-                for (int e = 0; e < N; ++e) v[k][e] = (v[k][e] - s2.x) * s2.y * w[e];
+                load_floats(w2, i, slice, w);
                 if (p.pre_beta != nullptr) {
-                    load_floats(b2 + i * N, w);
+                    float b[N];
+                    load_floats(b2, i, slice, b);
 #pragma unroll
-                    for (int e = 0; e < N; ++e) v[k][e] += w[e];
+                    for (int e = 0; e < N; ++e) v[k][e] = fmaf(fmaf(v[k][e], s2.y, shift2), w[e], b[e]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < N; ++e) v[k][e] = fmaf(v[k][e], s2.y, shift2) * w[e];
                 }
                 Chunk<T, N>::store_stream(static_cast<T*>(p.n) + base + static_cast<int64_t>(i) * N, v[k]);
             }
-        }
-        if (!released) {
-            __syncthreads();
-            release();
         }
         ring.next();
     }
@@ -756,18 +786,19 @@ norm_residual_backward_ring_kernel(const NormParams p, const RingPlan plan) {
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ RingSums<2> sums;
     __shared__ uint64_t full[kMaxStages];
+    __shared__ alignas(16) float4 stat[kMaxStages];  // the rows' statistics, beside their stages
     RingTeam<2> team{&sums, 0, static_cast<int>(blockDim.x) / kWarp, static_cast<int>(cluster_size()),
                      static_cast<int>(cluster_rank())};
     const int t = threadIdx.x, threads = blockDim.x;
-    const int row_packs = p.cols / N;
-    const int first = team.rank * plan.slice_packs;
-    const int count = min(plan.slice_packs, row_packs - first);
-    const int tile_bytes = plan.slice_packs * 16;
+    const int row_packs = p.cols / N, slice = plan.slice_packs;
+    const int first = team.rank * slice;
+    const int count = min(slice, row_packs - first);
     const int64_t teams = gridDim.x / team.cluster, id = blockIdx.x / team.cluster;
     const bool gate_each = p.gate != nullptr && p.rows_per_gate == 1;
     const bool gate_shared = p.gate != nullptr && !gate_each;
-    float* const w1 = reinterpret_cast<float*>(smem + static_cast<size_t>(plan.stages) * plan.tiles * tile_bytes);
-    float* const w2 = w1 + plan.slice_packs * N;
+    uint4* const stages = reinterpret_cast<uint4*>(smem);  // [stages][tiles][slice]
+    float4* const w1 = reinterpret_cast<float4*>(stages + static_cast<size_t>(plan.stages) * plan.tiles * slice);
+    float4* const w2 = w1 + slice * (N / 4);
     // Places of the tensors in a stage; an absent one has none.
     const int at_dn = 0, at_y = 1;
     const int at_h = p.dn != nullptr ? 2 : 0;
@@ -793,17 +824,18 @@ norm_residual_backward_ring_kernel(const NormParams p, const RingPlan plan) {
     auto request = [&](int stage) {
         if (ask_task >= p.tasks) return;
         const size_t at = (static_cast<size_t>(ask_row) * p.cols + static_cast<size_t>(first) * N) * sizeof(T);
-        unsigned char* to_smem = smem + static_cast<size_t>(stage) * plan.tiles * tile_bytes;
+        uint4* tile = stages + static_cast<size_t>(stage) * plan.tiles * slice;
         uint64_t* bar = &full[stage];
         const uint32_t bytes = static_cast<uint32_t>(count) * 16u;
-        mbar_expect_tx(bar, static_cast<uint32_t>(plan.tiles) * bytes);
+        mbar_expect_tx(bar, static_cast<uint32_t>(plan.tiles) * bytes + 16u);
+        bulk_g2s(&stat[stage], p.stats_in + 4 * ask_row, 16u, bar);
         if (p.dn != nullptr) {
-            bulk_g2s(to_smem + at_dn * tile_bytes, static_cast<const unsigned char*>(p.dn) + at, bytes, bar);
-            bulk_g2s(to_smem + at_y * tile_bytes, static_cast<const unsigned char*>(p.y_in) + at, bytes, bar);
+            bulk_g2s(tile + at_dn * slice, static_cast<const unsigned char*>(p.dn) + at, bytes, bar);
+            bulk_g2s(tile + at_y * slice, static_cast<const unsigned char*>(p.y_in) + at, bytes, bar);
         }
-        bulk_g2s(to_smem + at_h * tile_bytes, static_cast<const unsigned char*>(p.h) + at, bytes, bar);
-        if (p.dy != nullptr) bulk_g2s(to_smem + at_dy * tile_bytes, static_cast<const unsigned char*>(p.dy) + at, bytes, bar);
-        if (gate_each) bulk_g2s(to_smem + at_gate * tile_bytes, static_cast<const unsigned char*>(p.gate) + at, bytes, bar);
+        bulk_g2s(tile + at_h * slice, static_cast<const unsigned char*>(p.h) + at, bytes, bar);
+        if (p.dy != nullptr) bulk_g2s(tile + at_dy * slice, static_cast<const unsigned char*>(p.dy) + at, bytes, bar);
+        if (gate_each) bulk_g2s(tile + at_gate * slice, static_cast<const unsigned char*>(p.gate) + at, bytes, bar);
         if (++ask_row == ask_end) {
             ask_task += teams;
             if (ask_task < p.tasks) task_rows(ask_task, &ask_row, &ask_end);
@@ -820,11 +852,13 @@ norm_residual_backward_ring_kernel(const NormParams p, const RingPlan plan) {
         for (int e = 0; e < N; ++e) {
             s1[k][e] = a2[k][e] = 0.0f;
             s0[k][e % NB] = a3[k][e % NB] = 0.0f;
-            if (i < count) {
-                const int c = (first + i) * N + e;
-                w1[i * N + e] = p.block_scale * (p.post_gamma != nullptr ? p.post_gamma[c] : 1.0f);
-                w2[i * N + e] = p.pre_gamma != nullptr ? p.pre_gamma[c] : 1.0f;
-            }
+        }
+        if (i < count) {
+            float w[N];
+            fetch_floats(p.post_gamma, (first + i) * N, p.block_scale, w);
+            keep_floats(w1, i, slice, w);
+            fetch_floats(p.pre_gamma, (first + i) * N, 1.0f, w);
+            keep_floats(w2, i, slice, w);
         }
     }
     RingWait ring{full, plan.stages, 0, 0, false};
@@ -839,19 +873,19 @@ norm_residual_backward_ring_kernel(const NormParams p, const RingPlan plan) {
             for (int k = 0; k < PACKS; ++k) {
                 const int i = t + k * threads;
                 if (i >= count) continue;
-                float g[N];
+                float g[N], w[N];
                 Chunk<T, N>::load(static_cast<const T*>(p.gate) + group * p.cols + (first + i) * N, g);
+                gate_values(p.gate_act, g);
+                fetch_floats(p.post_gamma, (first + i) * N, p.block_scale, w);
 #pragma unroll
-                for (int e = 0; e < N; ++e) {
-                    const int c = (first + i) * N + e;
-                    w1[i * N + e] = p.block_scale * gate_value(p.gate_act, g[e]) * (p.post_gamma != nullptr ? p.post_gamma[c] : 1.0f);
-                }
+                for (int e = 0; e < N; ++e) w[e] *= g[e];
+                keep_floats(w1, i, slice, w);
             }
         }
         for (int64_t row = from; row < to; ++row) {
-            const float4 st = reinterpret_cast<const float4*>(p.stats_in)[row];
             ring.wait(p.error_flag);
-            const uint4* tile = reinterpret_cast<const uint4*>(smem + static_cast<size_t>(ring.stage) * plan.tiles * tile_bytes);
+            const uint4* tile = stages + static_cast<size_t>(ring.stage) * plan.tiles * slice;
+            const float4 st = stat[ring.stage];
             const int64_t base = row * p.cols + static_cast<int64_t>(first) * N;
             float d[PACKS][N], hat[PACKS][N];
             float level = 0.0f, along = 0.0f;
@@ -863,9 +897,9 @@ norm_residual_backward_ring_kernel(const NormParams p, const RingPlan plan) {
                     const int i = t + k * threads;
                     if (i < count) {
                         float w[N];
-                        unpack(tile[at_dn * plan.slice_packs + i], d[k], T{});
-                        unpack(tile[at_y * plan.slice_packs + i], hat[k], T{});
-                        load_floats(w2 + i * N, w);
+                        unpack(tile[at_dn * slice + i], d[k], T{});
+                        unpack(tile[at_y * slice + i], hat[k], T{});
+                        load_floats(w2, i, slice, w);
 #pragma unroll
                         for (int e = 0; e < N; ++e) {
                             hat[k][e] = fmaf(hat[k][e], st.w, shift);
@@ -898,35 +932,36 @@ norm_residual_backward_ring_kernel(const NormParams p, const RingPlan plan) {
                 if (i >= count) continue;
                 float w[N];
                 // D, and dx
-#pragma unroll
-                for (int e = 0; e < N; ++e) d[k][e] = st.w * (d[k][e] - level - hat[k][e] * along);
                 if (p.dy != nullptr) {
-                    unpack(tile[at_dy * plan.slice_packs + i], w, T{});
+                    unpack(tile[at_dy * slice + i], w, T{});
 #pragma unroll
-                    for (int e = 0; e < N; ++e) d[k][e] += w[e];
+                    for (int e = 0; e < N; ++e) d[k][e] = fmaf(st.w, fmaf(hat[k][e], -along, d[k][e] - level), w[e]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < N; ++e) d[k][e] = st.w * fmaf(hat[k][e], -along, d[k][e] - level);
                 }
                 if (p.dx != nullptr) {
 #pragma unroll
                     for (int e = 0; e < N; ++e) w[e] = p.residual_scale * d[k][e];
                     Chunk<T, N>::store_stream(static_cast<T*>(p.dx) + base + static_cast<int64_t>(i) * N, w);
                 }
-                unpack(tile[at_h * plan.slice_packs + i], hat[k], T{});
+                unpack(tile[at_h * slice + i], hat[k], T{});
 #pragma unroll
                 for (int e = 0; e < N; ++e) hat[k][e] = fmaf(hat[k][e], st.y, shift);
                 float scale[N];
-                load_floats(w1 + i * N, scale);  // block_scale * gamma (* a shared gate)
+                load_floats(w1, i, slice, scale);  // block_scale * gamma (* a shared gate)
                 if (gate_each) {
                     float a[N];
-                    unpack(tile[at_gate * plan.slice_packs + i], a, T{});
-#pragma unroll
-                    for (int e = 0; e < N; ++e) a[e] = gate_value(p.gate_act, a[e]);
+                    unpack(tile[at_gate * slice + i], a, T{});
+                    gate_values(p.gate_act, a);
                     if (p.dgate != nullptr) {
 #pragma unroll
                         for (int e = 0; e < N; ++e) {
                             float u = hat[k][e] * scale[e];
                             if (BETA && p.post_beta != nullptr) u += p.block_scale * p.post_beta[(first + i) * N + e];
-                            w[e] = d[k][e] * u * gate_slope(p.gate_act, a[e]);
+                            w[e] = d[k][e] * u;
                         }
+                        times_slope(p.gate_act, a, w);
                         Chunk<T, N>::store_stream(static_cast<T*>(p.dgate) + base + static_cast<int64_t>(i) * N, w);
                     }
 #pragma unroll
@@ -952,7 +987,7 @@ norm_residual_backward_ring_kernel(const NormParams p, const RingPlan plan) {
                     const int i = t + k * threads;
                     if (i >= count) continue;
 #pragma unroll
-                    for (int e = 0; e < N; ++e) d[k][e] = st.y * (d[k][e] - level - hat[k][e] * along);
+                    for (int e = 0; e < N; ++e) d[k][e] = st.y * fmaf(hat[k][e], -along, d[k][e] - level);
                     Chunk<T, N>::store_stream(static_cast<T*>(p.dh) + base + static_cast<int64_t>(i) * N, d[k]);
                 }
             }
@@ -966,16 +1001,22 @@ norm_residual_backward_ring_kernel(const NormParams p, const RingPlan plan) {
             const int i = t + k * threads;
             if (i >= count) continue;
             float g[N], a[N];
-            if (gate_shared) Chunk<T, N>::load(static_cast<const T*>(p.gate) + group * p.cols + (first + i) * N, g);
+            if (gate_shared) {
+                Chunk<T, N>::load(static_cast<const T*>(p.gate) + group * p.cols + (first + i) * N, a);
+                gate_values(p.gate_act, a);
+            } else {
+#pragma unroll
+                for (int e = 0; e < N; ++e) a[e] = 1.0f;
+            }
 #pragma unroll
             for (int e = 0; e < N; ++e) {
                 const int c = (first + i) * N + e;
-                a[e] = gate_shared ? gate_value(p.gate_act, g[e]) : 1.0f;
                 const float b = BETA ? s0[k][e % NB] : 0.0f;
+                g[e] = 0.0f;
                 if (gate_shared && p.dgate != nullptr) {
                     float u = (p.post_gamma != nullptr ? p.post_gamma[c] : 1.0f) * s1[k][e];
                     if (BETA && p.post_beta != nullptr) u += p.post_beta[c] * b;
-                    g[e] = p.block_scale * gate_slope(p.gate_act, a[e]) * u;
+                    g[e] = p.block_scale * u;
                 }
                 float* const pg = p.partial[0] != nullptr ? p.partial[0] + id * p.cols + c : nullptr;
                 float* const pb = p.partial[1] != nullptr ? p.partial[1] + id * p.cols + c : nullptr;
@@ -984,6 +1025,7 @@ norm_residual_backward_ring_kernel(const NormParams p, const RingPlan plan) {
                 s1[k][e] = 0.0f;
                 if (BETA) s0[k][e % NB] = 0.0f;
             }
+            times_slope(p.gate_act, a, g);
             if (gate_shared && p.dgate != nullptr) {
                 if (p.gate_partial != nullptr) {
 #pragma unroll
@@ -1082,21 +1124,21 @@ struct RingShape {
     size_t smem;
 };
 
-// A thread owns 8 columns, or 16 of a 16-bit type: forward beyond 4096 columns, backward without sums for the
-// betas (their registers).  Stages take what is left of the shared memory of an SM, shared by as many CTAs as
-// 1024 threads make (backward: 512, with 128 registers each).
+// A thread owns 8 columns, or 16 of a 16-bit type (two packs: the sums' instructions are shared by more
+// columns) -- but not for sums for the betas, whose registers would spill.  Stages take what is left of the
+// shared memory of an SM, shared by as many CTAs as 1024 threads make (backward: 512, with 128 registers each).
 RingShape ring_shape(int64_t cols, int dtype, int tiles, int weights, bool backward, bool beta) {
     RingShape r = {};
     const int n = 16 / static_cast<int>(dtype_bytes(dtype));
     if (cols % n != 0 || cols <= kWarpCols) return r;  // no whole packs, or a warp a row
     const int64_t packs = cols / n;
-    r.per_thread = dtype != FDL_F32 && (backward ? !beta : cols > 512 * 8) ? 16 : 8;
+    r.per_thread = dtype != FDL_F32 && !beta ? 16 : 8;
     r.cluster = 1;
     while (cols > static_cast<int64_t>(r.cluster) * 512 * r.per_thread) r.cluster *= 2;
     r.plan.slice_packs = static_cast<int>(ceil_div(packs, r.cluster));
     r.plan.tiles = tiles;
     r.threads = static_cast<int>(ceil_div(ceil_div(r.plan.slice_packs, r.per_thread / n), kWarp)) * kWarp;
-    const int budget = backward || r.per_thread == 16 ? 512 : 1024;
+    const int budget = backward ? 512 : 1024;
     r.blocks = budget / r.threads < 1 ? 1 : budget / r.threads > 16 ? 16 : budget / r.threads;
     const size_t fixed = static_cast<size_t>(r.plan.slice_packs) * n * 4 * weights;
     const size_t stage = static_cast<size_t>(r.plan.slice_packs) * 16 * tiles;
@@ -1218,24 +1260,15 @@ int launch_ring(K kernel, const NormParams& p, const RingShape& r, int64_t grid,
 int launch_ring_forward(int dtype, const NormParams& p, const RingShape& r, int64_t grid, cudaStream_t stream) {
     return with_dtype(dtype, [&](auto* tag) {
         using T = std::remove_pointer_t<decltype(tag)>;
-        if constexpr (kPack<T> == 8) {
-            if (r.per_thread == 16) return launch_ring(norm_residual_ring_kernel<T, 2>, p, r, grid, stream);
-        }
-        return launch_ring(norm_residual_ring_kernel<T, 8 / kPack<T>>, p, r, grid, stream);
+        return launch_ring(norm_residual_ring_kernel<T, 2>, p, r, grid, stream);
     });
 }
 
 int launch_ring_backward(int dtype, bool beta, const NormParams& p, const RingShape& r, int64_t grid, cudaStream_t stream) {
     return with_dtype(dtype, [&](auto* tag) {
         using T = std::remove_pointer_t<decltype(tag)>;
-        if constexpr (kPack<T> == 8) {
-            if (r.per_thread == 16) {
-                return beta ? launch_ring(norm_residual_backward_ring_kernel<T, 2, true>, p, r, grid, stream)
-                            : launch_ring(norm_residual_backward_ring_kernel<T, 2, false>, p, r, grid, stream);
-            }
-        }
         return beta ? launch_ring(norm_residual_backward_ring_kernel<T, 8 / kPack<T>, true>, p, r, grid, stream)
-                    : launch_ring(norm_residual_backward_ring_kernel<T, 8 / kPack<T>, false>, p, r, grid, stream);
+                    : launch_ring(norm_residual_backward_ring_kernel<T, 2, false>, p, r, grid, stream);
     });
 }
 
