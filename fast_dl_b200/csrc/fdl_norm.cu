@@ -158,6 +158,78 @@ __device__ __forceinline__ void times_slope(int act, const float (&a)[N], float 
     }
 }
 
+// Two floats in one instruction (a rounding each, as for one).
+__device__ __forceinline__ uint64_t bits2(float2 v) {
+    return static_cast<uint64_t>(__float_as_uint(v.x)) | static_cast<uint64_t>(__float_as_uint(v.y)) << 32;
+}
+__device__ __forceinline__ float2 floats2(uint64_t v) {
+    return make_float2(__uint_as_float(static_cast<uint32_t>(v)), __uint_as_float(static_cast<uint32_t>(v >> 32)));
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)), "l"(bits2(c)));
+    return floats2(d);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)));
+    return floats2(d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)));
+    return floats2(d);
+}
+
+// A 128-bit pack as pairs.
+__device__ __forceinline__ void unpack2(const uint4& u, float2 (&v)[2], float) {
+    v[0] = make_float2(__uint_as_float(u.x), __uint_as_float(u.y));
+    v[1] = make_float2(__uint_as_float(u.z), __uint_as_float(u.w));
+}
+__device__ __forceinline__ void unpack2(const uint4& u, float2 (&v)[4], __half) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+}
+__device__ __forceinline__ void unpack2(const uint4& u, float2 (&v)[4], __nv_bfloat16) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+}
+template <class T, int M>
+__device__ __forceinline__ void store_pairs(T* p, const float2 (&v)[M]) {
+    float f[2 * M];
+#pragma unroll
+    for (int e = 0; e < M; ++e) {
+        f[2 * e] = v[e].x;
+        f[2 * e + 1] = v[e].y;
+    }
+    __stcs(reinterpret_cast<uint4*>(p), repack(f, T{}));
+}
+template <int M>
+__device__ __forceinline__ void gate_pairs(int act, float2 (&g)[M]) {
+    float f[2 * M];
+#pragma unroll
+    for (int e = 0; e < M; ++e) {
+        f[2 * e] = g[e].x;
+        f[2 * e + 1] = g[e].y;
+    }
+    gate_values(act, f);
+#pragma unroll
+    for (int e = 0; e < M; ++e) g[e] = make_float2(f[2 * e], f[2 * e + 1]);
+}
+template <int M>
+__device__ __forceinline__ void times_slope_pairs(int act, const float2 (&a)[M], float2 (&v)[M]) {
+    if (act == FDL_GATE_SIGMOID) {
+#pragma unroll
+        for (int e = 0; e < M; ++e) v[e] = mul2(v[e], fma2(a[e], make_float2(-a[e].x, -a[e].y), a[e]));
+    } else if (act == FDL_GATE_TANH) {
+#pragma unroll
+        for (int e = 0; e < M; ++e) v[e] = mul2(v[e], fma2(a[e], make_float2(-a[e].x, -a[e].y), both(1.0f)));
+    }
+}
+
 template <int N, int PACKS>
 struct Owned {  // a thread's columns: PACKS chunks of N, a team's width apart
     int first, stride;
@@ -499,8 +571,10 @@ norm_residual_backward_kernel(const NormParams p) {
 //
 // For more rows than teams, on the 16-byte grid: one thread asks for whole row slices with bulk-async
 // copies, a few rows ahead of the row that the CTA works on, so the bytes in flight depend on neither
-// registers nor barriers.  gamma and beta (times the block's scale and a shared gate) lie in shared memory as
-// floats; a thread reads and writes only its own columns of them, so no barrier guards them.
+// registers nor barriers.  Arithmetic goes two floats an instruction: the kernels are near the issue limit.
+// Forward, gamma and beta come from L1 row by row (in shared memory they would take the place of a CTA).
+// Backward, with half the threads an SM, they lie in shared memory as floats (post_gamma times the block's
+// scale and a shared gate); a thread reads and writes only its own columns of them, so no barrier guards them.
 
 constexpr int kMaxStages = 4;
 
@@ -574,30 +648,35 @@ struct RingWait {
 
 // The floats of pack i, kept as N / 4 arrays of 128-bit groups so that lanes next to each other read next
 // to each other.
-template <int N>
-__device__ __forceinline__ void load_floats(const float4* w, int i, int packs, float (&v)[N]) {
+template <int M>
+__device__ __forceinline__ void load_floats(const float4* w, int i, int packs, float2 (&v)[M]) {
 #pragma unroll
-    for (int q = 0; q < N / 4; ++q) {
+    for (int q = 0; q < M / 2; ++q) {
         const float4 f = w[q * packs + i];
-        v[4 * q] = f.x; v[4 * q + 1] = f.y; v[4 * q + 2] = f.z; v[4 * q + 3] = f.w;
+        v[2 * q] = make_float2(f.x, f.y);
+        v[2 * q + 1] = make_float2(f.z, f.w);
     }
 }
-template <int N>
-__device__ __forceinline__ void keep_floats(float4* w, int i, int packs, const float (&v)[N]) {
+template <int M>
+__device__ __forceinline__ void keep_floats(float4* w, int i, int packs, const float2 (&v)[M]) {
 #pragma unroll
-    for (int q = 0; q < N / 4; ++q) w[q * packs + i] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+    for (int q = 0; q < M / 2; ++q) w[q * packs + i] = make_float4(v[2 * q].x, v[2 * q].y, v[2 * q + 1].x, v[2 * q + 1].y);
 }
-// scale * w[col ...], or scale where there is no w.
-template <int N>
-__device__ __forceinline__ void fetch_floats(const float* w, int col, float scale, float (&v)[N]) {
+// w[col ...] (on the 16-byte grid), or ones where there is no w.
+template <int M>
+__device__ __forceinline__ void fetch_floats(const float* w, int col, float2 (&v)[M]) {
 #pragma unroll
-    for (int e = 0; e < N; ++e) v[e] = w != nullptr ? scale * w[col + e] : scale;
+    for (int q = 0; q < M / 2; ++q) {
+        const float4 f = w != nullptr ? __ldg(reinterpret_cast<const float4*>(w + col) + q) : make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+        v[2 * q] = make_float2(f.x, f.y);
+        v[2 * q + 1] = make_float2(f.z, f.w);
+    }
 }
 
 template <class T, int PACKS>
 __global__ void __launch_bounds__(512, 2)
 norm_residual_ring_kernel(const NormParams p, const RingPlan plan) {
-    constexpr int N = kPack<T>;
+    constexpr int N = kPack<T>, M = N / 2;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ RingSums<1> sums;
     __shared__ uint64_t full[kMaxStages];
@@ -608,14 +687,10 @@ norm_residual_ring_kernel(const NormParams p, const RingPlan plan) {
     const int first = team.rank * slice;
     const int count = min(slice, row_packs - first);
     const int64_t teams = gridDim.x / team.cluster, id = blockIdx.x / team.cluster;
-    // A contiguous run of rows a team: a shared gate changes seldom.
     const int64_t from = p.rows * id / teams, to = p.rows * (id + 1) / teams;
     const bool gate_each = p.gate != nullptr && p.rows_per_gate == 1;
+    const bool gate_shared = p.gate != nullptr && !gate_each;
     uint4* const stages = reinterpret_cast<uint4*>(smem);  // [stages][tiles][slice]
-    float4* const w1 = reinterpret_cast<float4*>(stages + static_cast<size_t>(plan.stages) * plan.tiles * slice);
-    float4* const w2 = w1 + slice * (N / 4);
-    float4* const b1 = w2 + slice * (N / 4);
-    float4* const b2 = p.post_beta != nullptr ? b1 + slice * (N / 4) : b1;
     if (t == 0) {
         for (int s = 0; s < plan.stages; ++s) mbar_init(&full[s], 1);
         fence_mbar_init();
@@ -634,114 +709,93 @@ norm_residual_ring_kernel(const NormParams p, const RingPlan plan) {
     if (t == 0) {
         for (int s = 0; s < plan.stages && from + s < to; ++s) request(from + s, s);
     }
-    auto weigh = [&](float (&scale)[N], int i) {  // post_gamma, post_beta times the block's scale (and a shared gate)
-        float w[N];
-        fetch_floats(p.post_gamma, (first + i) * N, 1.0f, w);
-#pragma unroll
-        for (int e = 0; e < N; ++e) w[e] *= scale[e];
-        keep_floats(w1, i, slice, w);
-        if (p.post_beta != nullptr) {
-            fetch_floats(p.post_beta, (first + i) * N, 1.0f, w);
-#pragma unroll
-            for (int e = 0; e < N; ++e) w[e] *= scale[e];
-            keep_floats(b1, i, slice, w);
-        }
-    };
-#pragma unroll
-    for (int k = 0; k < PACKS; ++k) {
-        const int i = t + k * threads;
-        if (i >= count) continue;
-        float w[N];
-#pragma unroll
-        for (int e = 0; e < N; ++e) w[e] = p.block_scale;
-        weigh(w, i);
-        fetch_floats(p.pre_gamma, (first + i) * N, 1.0f, w);
-        keep_floats(w2, i, slice, w);
-        if (p.pre_beta != nullptr) {
-            fetch_floats(p.pre_beta, (first + i) * N, 1.0f, w);
-            keep_floats(b2, i, slice, w);
-        }
-    }
     RingWait ring{full, plan.stages, 0, 0, false};
     const float inv = 1.0f / static_cast<float>(p.cols);
-    int64_t group = -1;
-    for (int64_t row = from; row < to; ++row) {
-        if (p.gate != nullptr && !gate_each && row / p.rows_per_gate != group) {  // another shared gate row
-            group = row / p.rows_per_gate;
-#pragma unroll
-            for (int k = 0; k < PACKS; ++k) {
-                const int i = t + k * threads;
-                if (i >= count) continue;
-                float g[N];
-                Chunk<T, N>::load(static_cast<const T*>(p.gate) + group * p.cols + (first + i) * N, g);
-                gate_values(p.gate_act, g);
-#pragma unroll
-                for (int e = 0; e < N; ++e) g[e] *= p.block_scale;
-                weigh(g, i);
-            }
-        }
+    const float2 residual = both(p.residual_scale);
+    // This thread's first column in the current row, and of the shared gate's row.
+    const int64_t start = from * p.cols + static_cast<int64_t>(first + t) * N;
+    T* y = static_cast<T*>(p.y) + start;
+    T* n = p.n != nullptr ? static_cast<T*>(p.n) + start : nullptr;
+    const T* gate = nullptr;
+    int64_t gate_left = 0;  // rows that the gate's row still serves
+    if (gate_shared && from < to) {
+        const int64_t group = from / p.rows_per_gate;
+        gate = static_cast<const T*>(p.gate) + group * p.cols + static_cast<int64_t>(first + t) * N;
+        gate_left = (group + 1) * p.rows_per_gate - from;
+    }
+    for (int64_t row = from; row < to; ++row, y += p.cols, n += p.n != nullptr ? p.cols : 0) {
         ring.wait(p.error_flag);
-        const uint4* tile = stages + static_cast<size_t>(ring.stage) * plan.tiles * slice;
-        float v[PACKS][N];
+        const uint4* tile = stages + ring.stage * plan.tiles * slice;
+        float2 v[PACKS][M];
 #pragma unroll
         for (int k = 0; k < PACKS; ++k) {
             const int i = t + k * threads;
-            unpack(i < count ? tile[i] : make_uint4(0, 0, 0, 0), v[k], T{});
+            unpack2(i < count ? tile[i] : make_uint4(0, 0, 0, 0), v[k], T{});
         }
         auto moments = [&](int kind) {
             if (kind == FDL_NORM_NONE) return make_float2(0.0f, 1.0f);
             float mean = 0.0f;
+            float2 q2 = both(0.0f);
             if (kind == FDL_NORM_LAYER) {
-                float s[1] = {0.0f};
+                float2 s2 = both(0.0f);
 #pragma unroll
                 for (int k = 0; k < PACKS; ++k) {
 #pragma unroll
-                    for (int e = 0; e < N; ++e) s[0] += v[k][e];
+                    for (int e = 0; e < M; ++e) s2 = add2(s2, v[k][e]);
                 }
+                float s[1] = {s2.x + s2.y};
                 team.sum(s);
                 mean = s[0] * inv;
-            }
-            float q[1] = {0.0f};
 #pragma unroll
-            for (int k = 0; k < PACKS; ++k) {
-                if (t + k * threads < count) {
+                for (int k = 0; k < PACKS; ++k) {
+                    if (t + k * threads >= count) continue;
 #pragma unroll
-                    for (int e = 0; e < N; ++e) q[0] = fmaf(v[k][e] - mean, v[k][e] - mean, q[0]);
+                    for (int e = 0; e < M; ++e) {
+                        const float2 c = add2(v[k][e], both(-mean));
+                        q2 = fma2(c, c, q2);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < PACKS; ++k) {
+#pragma unroll
+                    for (int e = 0; e < M; ++e) q2 = fma2(v[k][e], v[k][e], q2);
                 }
             }
+            float q[1] = {q2.x + q2.y};
             team.sum(q);
-            return make_float2(mean, 1.0f / sqrtf(fmaf(q[0], inv, p.eps)));
+            return make_float2(mean, rsqrtf(fmaf(q[0], inv, p.eps)));
         };
         const float2 s1 = moments(p.post_kind);
-        const int64_t base = row * p.cols + static_cast<int64_t>(first) * N;
-        const float shift1 = -s1.x * s1.y;
+        // (h - mean) * r * gamma * block_scale: the scale goes into r
+        const float2 r1 = both(s1.y * p.block_scale), shift1 = both(-s1.x * s1.y * p.block_scale);
 #pragma unroll
         for (int k = 0; k < PACKS; ++k) {
             const int i = t + k * threads;
             if (i >= count) continue;
-            float w[N];
-            load_floats(w1, i, slice, w);
+            float2 w[M];
+#pragma unroll
+            for (int e = 0; e < M; ++e) v[k][e] = fma2(v[k][e], r1, shift1);
+            if (p.post_gamma != nullptr) {
+                fetch_floats(p.post_gamma, (first + i) * N, w);
+#pragma unroll
+                for (int e = 0; e < M; ++e) v[k][e] = mul2(v[k][e], w[e]);
+            }
             if (p.post_beta != nullptr) {
-                float b[N];
-                load_floats(b1, i, slice, b);
+                fetch_floats(p.post_beta, (first + i) * N, w);
 #pragma unroll
-                for (int e = 0; e < N; ++e) v[k][e] = fmaf(fmaf(v[k][e], s1.y, shift1), w[e], b[e]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < N; ++e) v[k][e] = fmaf(v[k][e], s1.y, shift1) * w[e];
+                for (int e = 0; e < M; ++e) v[k][e] = fma2(both(p.block_scale), w[e], v[k][e]);
             }
-            float x[N];
-            unpack(tile[slice + i], x, T{});
-            if (gate_each) {
-                unpack(tile[2 * slice + i], w, T{});
-                gate_values(p.gate_act, w);
+            if (p.gate != nullptr) {
+                unpack2(gate_each ? tile[2 * slice + i] : __ldg(reinterpret_cast<const uint4*>(gate) + k * threads), w, T{});
+                gate_pairs(p.gate_act, w);
 #pragma unroll
-                for (int e = 0; e < N; ++e) v[k][e] = fmaf(v[k][e], w[e], p.residual_scale * x[e]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < N; ++e) v[k][e] = fmaf(p.residual_scale, x[e], v[k][e]);
+                for (int e = 0; e < M; ++e) v[k][e] = mul2(v[k][e], w[e]);
             }
-            Chunk<T, N>::store_stream(static_cast<T*>(p.y) + base + static_cast<int64_t>(i) * N, v[k]);
+            unpack2(tile[slice + i], w, T{});
+#pragma unroll
+            for (int e = 0; e < M; ++e) v[k][e] = fma2(residual, w[e], v[k][e]);
+            store_pairs(y + k * threads * N, v[k]);
         }
         const float2 s2 = moments(p.pre_kind);
         if (p.pre_kind == FDL_NORM_NONE) __syncthreads();
@@ -751,24 +805,30 @@ norm_residual_ring_kernel(const NormParams p, const RingPlan plan) {
             reinterpret_cast<float4*>(p.stats)[row] = make_float4(s1.x, s1.y, s2.x, s2.y);
         }
         if (p.n != nullptr) {
-            const float shift2 = -s2.x * s2.y;
+            const float2 r2 = both(s2.y), shift2 = both(-s2.x * s2.y);
 #pragma unroll
             for (int k = 0; k < PACKS; ++k) {
                 const int i = t + k * threads;
                 if (i >= count) continue;
-                float w[N];
-                load_floats(w2, i, slice, w);
-                if (p.pre_beta != nullptr) {
-                    float b[N];
-                    load_floats(b2, i, slice, b);
+                float2 w[M];
 #pragma unroll
-                    for (int e = 0; e < N; ++e) v[k][e] = fmaf(fmaf(v[k][e], s2.y, shift2), w[e], b[e]);
-                } else {
+                for (int e = 0; e < M; ++e) v[k][e] = fma2(v[k][e], r2, shift2);
+                if (p.pre_gamma != nullptr) {
+                    fetch_floats(p.pre_gamma, (first + i) * N, w);
 #pragma unroll
-                    for (int e = 0; e < N; ++e) v[k][e] = fmaf(v[k][e], s2.y, shift2) * w[e];
+                    for (int e = 0; e < M; ++e) v[k][e] = mul2(v[k][e], w[e]);
                 }
-                Chunk<T, N>::store_stream(static_cast<T*>(p.n) + base + static_cast<int64_t>(i) * N, v[k]);
+                if (p.pre_beta != nullptr) {
+                    fetch_floats(p.pre_beta, (first + i) * N, w);
+#pragma unroll
+                    for (int e = 0; e < M; ++e) v[k][e] = add2(v[k][e], w[e]);
+                }
+                store_pairs(n + k * threads * N, v[k]);
             }
+        }
+        if (gate_shared && --gate_left == 0) {
+            gate += p.cols;
+            gate_left = p.rows_per_gate;
         }
         ring.next();
     }
@@ -781,8 +841,8 @@ norm_residual_ring_kernel(const NormParams p, const RingPlan plan) {
 template <class T, int PACKS, bool BETA>
 __global__ void __launch_bounds__(512, 1)
 norm_residual_backward_ring_kernel(const NormParams p, const RingPlan plan) {
-    constexpr int N = kPack<T>;
-    constexpr int NB = BETA ? N : 1;
+    constexpr int N = kPack<T>, M = N / 2;
+    constexpr int MB = BETA ? M : 1;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ RingSums<2> sums;
     __shared__ uint64_t full[kMaxStages];
@@ -844,20 +904,22 @@ norm_residual_backward_ring_kernel(const NormParams p, const RingPlan plan) {
     if (t == 0) {
         for (int s = 0; s < plan.stages; ++s) request(s);
     }
-    float s1[PACKS][N], s0[PACKS][NB], a2[PACKS][N], a3[PACKS][NB];
+    float2 s1[PACKS][M], s0[PACKS][MB], a2[PACKS][M], a3[PACKS][MB];
 #pragma unroll
     for (int k = 0; k < PACKS; ++k) {
         const int i = t + k * threads;
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-            s1[k][e] = a2[k][e] = 0.0f;
-            s0[k][e % NB] = a3[k][e % NB] = 0.0f;
+        for (int e = 0; e < M; ++e) {
+            s1[k][e] = a2[k][e] = both(0.0f);
+            s0[k][e % MB] = a3[k][e % MB] = both(0.0f);
         }
         if (i < count) {
-            float w[N];
-            fetch_floats(p.post_gamma, (first + i) * N, p.block_scale, w);
+            float2 w[M];
+            fetch_floats(p.post_gamma, (first + i) * N, w);
+#pragma unroll
+            for (int e = 0; e < M; ++e) w[e] = mul2(w[e], both(p.block_scale));
             keep_floats(w1, i, slice, w);
-            fetch_floats(p.pre_gamma, (first + i) * N, 1.0f, w);
+            fetch_floats(p.pre_gamma, (first + i) * N, w);
             keep_floats(w2, i, slice, w);
         }
     }
@@ -873,12 +935,12 @@ norm_residual_backward_ring_kernel(const NormParams p, const RingPlan plan) {
             for (int k = 0; k < PACKS; ++k) {
                 const int i = t + k * threads;
                 if (i >= count) continue;
-                float g[N], w[N];
-                Chunk<T, N>::load(static_cast<const T*>(p.gate) + group * p.cols + (first + i) * N, g);
-                gate_values(p.gate_act, g);
-                fetch_floats(p.post_gamma, (first + i) * N, p.block_scale, w);
+                float2 g[M], w[M];
+                unpack2(*reinterpret_cast<const uint4*>(static_cast<const T*>(p.gate) + group * p.cols + (first + i) * N), g, T{});
+                gate_pairs(p.gate_act, g);
+                fetch_floats(p.post_gamma, (first + i) * N, w);
 #pragma unroll
-                for (int e = 0; e < N; ++e) w[e] *= g[e];
+                for (int e = 0; e < M; ++e) w[e] = mul2(mul2(w[e], both(p.block_scale)), g[e]);
                 keep_floats(w1, i, slice, w);
             }
         }
@@ -887,33 +949,34 @@ norm_residual_backward_ring_kernel(const NormParams p, const RingPlan plan) {
             const uint4* tile = stages + static_cast<size_t>(ring.stage) * plan.tiles * slice;
             const float4 st = stat[ring.stage];
             const int64_t base = row * p.cols + static_cast<int64_t>(first) * N;
-            float d[PACKS][N], hat[PACKS][N];
+            float2 d[PACKS][M], hat[PACKS][M];
             float level = 0.0f, along = 0.0f;
             if (p.dn != nullptr) {
-                float s[2] = {0.0f, 0.0f};
-                const float shift = -st.z * st.w;
+                float2 sd = both(0.0f), sh = both(0.0f);
+                const float2 r = both(st.w), shift = both(-st.z * st.w);
 #pragma unroll
                 for (int k = 0; k < PACKS; ++k) {
                     const int i = t + k * threads;
                     if (i < count) {
-                        float w[N];
-                        unpack(tile[at_dn * slice + i], d[k], T{});
-                        unpack(tile[at_y * slice + i], hat[k], T{});
+                        float2 w[M];
+                        unpack2(tile[at_dn * slice + i], d[k], T{});
+                        unpack2(tile[at_y * slice + i], hat[k], T{});
                         load_floats(w2, i, slice, w);
 #pragma unroll
-                        for (int e = 0; e < N; ++e) {
-                            hat[k][e] = fmaf(hat[k][e], st.w, shift);
-                            a2[k][e] = fmaf(d[k][e], hat[k][e], a2[k][e]);
-                            if (BETA) a3[k][e % NB] += d[k][e];
-                            d[k][e] *= w[e];
-                            s[0] += d[k][e];
-                            s[1] = fmaf(d[k][e], hat[k][e], s[1]);
+                        for (int e = 0; e < M; ++e) {
+                            hat[k][e] = fma2(hat[k][e], r, shift);
+                            a2[k][e] = fma2(d[k][e], hat[k][e], a2[k][e]);
+                            if (BETA) a3[k][e % MB] = add2(a3[k][e % MB], d[k][e]);
+                            d[k][e] = mul2(d[k][e], w[e]);
+                            sd = add2(sd, d[k][e]);
+                            sh = fma2(d[k][e], hat[k][e], sh);
                         }
                     } else {
 #pragma unroll
-                        for (int e = 0; e < N; ++e) d[k][e] = hat[k][e] = 0.0f;
+                        for (int e = 0; e < M; ++e) d[k][e] = hat[k][e] = both(0.0f);
                     }
                 }
+                float s[2] = {sd.x + sd.y, sh.x + sh.y};
                 team.sum(s);
                 level = p.pre_kind == FDL_NORM_LAYER ? s[0] * inv : 0.0f;
                 along = s[1] * inv;
@@ -921,74 +984,81 @@ norm_residual_backward_ring_kernel(const NormParams p, const RingPlan plan) {
 #pragma unroll
                 for (int k = 0; k < PACKS; ++k) {
 #pragma unroll
-                    for (int e = 0; e < N; ++e) d[k][e] = hat[k][e] = 0.0f;
+                    for (int e = 0; e < M; ++e) d[k][e] = hat[k][e] = both(0.0f);
                 }
             }
-            float s[2] = {0.0f, 0.0f};
-            const float shift = -st.x * st.y;
+            float2 sd = both(0.0f), sh = both(0.0f);
+            {
+                const float2 r1 = both(st.y), shift = both(-st.x * st.y), r2 = both(st.w);
+                const float2 down = both(-along), lower = both(-level);
 #pragma unroll
-            for (int k = 0; k < PACKS; ++k) {
-                const int i = t + k * threads;
-                if (i >= count) continue;
-                float w[N];
-                // D, and dx
-                if (p.dy != nullptr) {
-                    unpack(tile[at_dy * slice + i], w, T{});
+                for (int k = 0; k < PACKS; ++k) {
+                    const int i = t + k * threads;
+                    if (i >= count) continue;
+                    float2 w[M];
+                    // D, and dx
+                    if (p.dy != nullptr) {
+                        unpack2(tile[at_dy * slice + i], w, T{});
 #pragma unroll
-                    for (int e = 0; e < N; ++e) d[k][e] = fmaf(st.w, fmaf(hat[k][e], -along, d[k][e] - level), w[e]);
-                } else {
+                        for (int e = 0; e < M; ++e) d[k][e] = fma2(r2, fma2(hat[k][e], down, add2(d[k][e], lower)), w[e]);
+                    } else {
 #pragma unroll
-                    for (int e = 0; e < N; ++e) d[k][e] = st.w * fmaf(hat[k][e], -along, d[k][e] - level);
-                }
-                if (p.dx != nullptr) {
+                        for (int e = 0; e < M; ++e) d[k][e] = mul2(r2, fma2(hat[k][e], down, add2(d[k][e], lower)));
+                    }
+                    if (p.dx != nullptr) {
 #pragma unroll
-                    for (int e = 0; e < N; ++e) w[e] = p.residual_scale * d[k][e];
-                    Chunk<T, N>::store_stream(static_cast<T*>(p.dx) + base + static_cast<int64_t>(i) * N, w);
-                }
-                unpack(tile[at_h * slice + i], hat[k], T{});
+                        for (int e = 0; e < M; ++e) w[e] = mul2(both(p.residual_scale), d[k][e]);
+                        store_pairs(static_cast<T*>(p.dx) + base + static_cast<int64_t>(i) * N, w);
+                    }
+                    unpack2(tile[at_h * slice + i], hat[k], T{});
 #pragma unroll
-                for (int e = 0; e < N; ++e) hat[k][e] = fmaf(hat[k][e], st.y, shift);
-                float scale[N];
-                load_floats(w1, i, slice, scale);  // block_scale * gamma (* a shared gate)
-                if (gate_each) {
-                    float a[N];
-                    unpack(tile[at_gate * slice + i], a, T{});
-                    gate_values(p.gate_act, a);
-                    if (p.dgate != nullptr) {
+                    for (int e = 0; e < M; ++e) hat[k][e] = fma2(hat[k][e], r1, shift);
+                    float2 scale[M];
+                    load_floats(w1, i, slice, scale);  // block_scale * gamma (* a shared gate)
+                    if (gate_each) {
+                        float2 a[M];
+                        unpack2(tile[at_gate * slice + i], a, T{});
+                        gate_pairs(p.gate_act, a);
+                        if (p.dgate != nullptr) {
+                            if (BETA && p.post_beta != nullptr) {
+                                fetch_floats(p.post_beta, (first + i) * N, w);
 #pragma unroll
-                        for (int e = 0; e < N; ++e) {
-                            float u = hat[k][e] * scale[e];
-                            if (BETA && p.post_beta != nullptr) u += p.block_scale * p.post_beta[(first + i) * N + e];
-                            w[e] = d[k][e] * u;
+                                for (int e = 0; e < M; ++e) w[e] = mul2(d[k][e], fma2(hat[k][e], scale[e], mul2(both(p.block_scale), w[e])));
+                            } else {
+#pragma unroll
+                                for (int e = 0; e < M; ++e) w[e] = mul2(d[k][e], mul2(hat[k][e], scale[e]));
+                            }
+                            times_slope_pairs(p.gate_act, a, w);
+                            store_pairs(static_cast<T*>(p.dgate) + base + static_cast<int64_t>(i) * N, w);
                         }
-                        times_slope(p.gate_act, a, w);
-                        Chunk<T, N>::store_stream(static_cast<T*>(p.dgate) + base + static_cast<int64_t>(i) * N, w);
+#pragma unroll
+                        for (int e = 0; e < M; ++e) d[k][e] = mul2(d[k][e], a[e]);
                     }
 #pragma unroll
-                    for (int e = 0; e < N; ++e) d[k][e] *= a[e];
-                }
-#pragma unroll
-                for (int e = 0; e < N; ++e) {
-                    s1[k][e] = fmaf(d[k][e], hat[k][e], s1[k][e]);
-                    if (BETA) s0[k][e % NB] += d[k][e];
-                    d[k][e] *= scale[e];
-                    s[0] += d[k][e];
-                    s[1] = fmaf(d[k][e], hat[k][e], s[1]);
+                    for (int e = 0; e < M; ++e) {
+                        s1[k][e] = fma2(d[k][e], hat[k][e], s1[k][e]);
+                        if (BETA) s0[k][e % MB] = add2(s0[k][e % MB], d[k][e]);
+                        d[k][e] = mul2(d[k][e], scale[e]);
+                        sd = add2(sd, d[k][e]);
+                        sh = fma2(d[k][e], hat[k][e], sh);
+                    }
                 }
             }
+            float s[2] = {sd.x + sd.y, sh.x + sh.y};
             if (p.post_kind != FDL_NORM_NONE) team.sum(s);
             else __syncthreads();
             if (t == 0 && !ring.failed) request(ring.stage);  // everybody has read the stage
             if (p.dh != nullptr) {
                 level = p.post_kind == FDL_NORM_LAYER ? s[0] * inv : 0.0f;
                 along = p.post_kind != FDL_NORM_NONE ? s[1] * inv : 0.0f;
+                const float2 r1 = both(st.y), down = both(-along), lower = both(-level);
 #pragma unroll
                 for (int k = 0; k < PACKS; ++k) {
                     const int i = t + k * threads;
                     if (i >= count) continue;
 #pragma unroll
-                    for (int e = 0; e < N; ++e) d[k][e] = st.y * fmaf(hat[k][e], -along, d[k][e] - level);
-                    Chunk<T, N>::store_stream(static_cast<T*>(p.dh) + base + static_cast<int64_t>(i) * N, d[k]);
+                    for (int e = 0; e < M; ++e) d[k][e] = mul2(r1, fma2(hat[k][e], down, add2(d[k][e], lower)));
+                    store_pairs(static_cast<T*>(p.dh) + base + static_cast<int64_t>(i) * N, d[k]);
                 }
             }
             ring.next();
@@ -1011,19 +1081,23 @@ norm_residual_backward_ring_kernel(const NormParams p, const RingPlan plan) {
 #pragma unroll
             for (int e = 0; e < N; ++e) {
                 const int c = (first + i) * N + e;
-                const float b = BETA ? s0[k][e % NB] : 0.0f;
+                const float f = e % 2 == 0 ? s1[k][e / 2].x : s1[k][e / 2].y;
+                const float b = !BETA ? 0.0f : e % 2 == 0 ? s0[k][e / 2 % MB].x : s0[k][e / 2 % MB].y;
                 g[e] = 0.0f;
                 if (gate_shared && p.dgate != nullptr) {
-                    float u = (p.post_gamma != nullptr ? p.post_gamma[c] : 1.0f) * s1[k][e];
+                    float u = (p.post_gamma != nullptr ? p.post_gamma[c] : 1.0f) * f;
                     if (BETA && p.post_beta != nullptr) u += p.post_beta[c] * b;
                     g[e] = p.block_scale * u;
                 }
                 float* const pg = p.partial[0] != nullptr ? p.partial[0] + id * p.cols + c : nullptr;
                 float* const pb = p.partial[1] != nullptr ? p.partial[1] + id * p.cols + c : nullptr;
-                if (pg != nullptr) *pg = (flushed ? *pg : 0.0f) + p.block_scale * a[e] * s1[k][e];
+                if (pg != nullptr) *pg = (flushed ? *pg : 0.0f) + p.block_scale * a[e] * f;
                 if (pb != nullptr) *pb = (flushed ? *pb : 0.0f) + p.block_scale * a[e] * b;
-                s1[k][e] = 0.0f;
-                if (BETA) s0[k][e % NB] = 0.0f;
+            }
+#pragma unroll
+            for (int e = 0; e < M; ++e) {
+                s1[k][e] = both(0.0f);
+                if (BETA) s0[k][e % MB] = both(0.0f);
             }
             times_slope(p.gate_act, a, g);
             if (gate_shared && p.dgate != nullptr) {
@@ -1044,8 +1118,8 @@ norm_residual_backward_ring_kernel(const NormParams p, const RingPlan plan) {
 #pragma unroll
         for (int e = 0; e < N; ++e) {
             const int64_t c = id * p.cols + (first + i) * N + e;
-            if (p.partial[2] != nullptr) p.partial[2][c] = a2[k][e];
-            if (p.partial[3] != nullptr) p.partial[3][c] = BETA ? a3[k][e % NB] : 0.0f;
+            if (p.partial[2] != nullptr) p.partial[2][c] = e % 2 == 0 ? a2[k][e / 2].x : a2[k][e / 2].y;
+            if (BETA && p.partial[3] != nullptr) p.partial[3][c] = e % 2 == 0 ? a3[k][e / 2 % MB].x : a3[k][e / 2 % MB].y;
             if (!flushed) {  // a team without a task
                 if (p.partial[0] != nullptr) p.partial[0][c] = 0.0f;
                 if (p.partial[1] != nullptr) p.partial[1][c] = 0.0f;
@@ -1307,9 +1381,8 @@ int fdl_norm_residual(const void* x, const void* h, const void* gate, int64_t ga
     p.residual_scale = residual_scale; p.block_scale = block_scale; p.eps = eps;
     const bool vec = packs_fit(dtype, cols, {x, h, gate, y, n});
     const Shape s = shape_of(cols);
-    if (vec) {
-        const int weights = 2 + (post_beta != nullptr) + (pre_beta != nullptr);
-        const RingShape r = ring_shape(cols, dtype, 2 + (gate != nullptr && gate_rows == rows), weights, false, false);
+    if (vec && aligned16(post_gamma) && aligned16(post_beta) && aligned16(pre_gamma) && aligned16(pre_beta)) {
+        const RingShape r = ring_shape(cols, dtype, 2 + (gate != nullptr && gate_rows == rows), 0, false, false);
         const int64_t teams = r.plan.stages >= 2 ? static_cast<int64_t>(info->sm_count) * r.blocks / r.cluster : rows;
         if (rows > teams) {
             status = error_flag_device_ptr(&p.error_flag);
@@ -1392,7 +1465,7 @@ int fdl_norm_residual_backward(const void* dy, const void* dn, const void* y, co
     const bool beta = dpost_beta != nullptr || dpre_beta != nullptr || (post_beta != nullptr && dgate != nullptr);
     const int tiles = 1 + (dn != nullptr ? 2 : 0) + (dy != nullptr) + (gate != nullptr && gate_rows == rows);
     const RingShape r = ring_shape(cols, dtype, tiles, 2, true, beta);
-    const bool ring = vec && r.plan.stages >= 2;
+    const bool ring = vec && r.plan.stages >= 2 && aligned16(post_gamma) && aligned16(post_beta) && aligned16(pre_gamma);
     const BackwardPlan b = backward_plan(rows, cols, gate_rows, info->sm_count, ring ? &r : nullptr);
     NormParams p = {};
     p.dy = dy; p.dn = dn; p.y_in = y; p.h = h; p.stats_in = stats; p.gate = gate;
