@@ -160,10 +160,14 @@ __device__ __forceinline__ void times_slope(int act, const float (&a)[N], float 
 
 // Two floats in one instruction (a rounding each, as for one).
 __device__ __forceinline__ uint64_t bits2(float2 v) {
-    return static_cast<uint64_t>(__float_as_uint(v.x)) | static_cast<uint64_t>(__float_as_uint(v.y)) << 32;
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y));
+    return r;
 }
 __device__ __forceinline__ float2 floats2(uint64_t v) {
-    return make_float2(__uint_as_float(static_cast<uint32_t>(v)), __uint_as_float(static_cast<uint32_t>(v >> 32)));
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
 }
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
