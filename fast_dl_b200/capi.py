@@ -359,67 +359,89 @@ def take_device_error() -> None:
 # too, so that a captured call replays on memory of its own).
 
 
-_dtype_codes = None
+# A call for one token or one sequence takes the GPU a few microseconds, so the checks are written to take few:
+# one combined test a tensor, its parts told apart only when it fails.
+
+_torch = None
+_dtype_codes = {}
+_raw_stream = None
 
 
-def _dtype_code(t, what):
-    global _dtype_codes
-    if _dtype_codes is None:
-        import torch
-        _dtype_codes = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+def _load_torch():
+    global _torch, _raw_stream
+    import torch
+    _dtype_codes.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+    # the current stream's handle without a Stream object around it, where this torch has that
+    _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+        lambda device: torch.cuda.current_stream(device).cuda_stream)
+    _torch = torch
+    return torch
+
+
+def _device_of(where, t):
+    """The current CUDA device, if `t` is on it."""
+    torch = _torch or _load_torch()
+    if t.is_cuda:
+        device = torch.cuda.current_device()
+        if t.get_device() == device:
+            return device
+    raise ValueError(f"{where}: expected tensors on the current CUDA device, got {t.device}")
+
+
+def _dtype_code(where, t):
     code = _dtype_codes.get(t.dtype)
     if code is None:
-        raise ValueError(f"{what}: expected float32, float16 or bfloat16, got {t.dtype}")
+        raise ValueError(f"{where}: expected float32, float16 or bfloat16, got {t.dtype}")
     return code
 
 
-def _here(t, what, shape=None, dtype=None, contiguous=True):
-    """`t`, if it is a tensor on the current CUDA device of this shape and type."""
-    import torch
-    if not t.is_cuda or t.device.index != torch.cuda.current_device():
-        raise ValueError(f"{what}: expected a tensor on the current CUDA device, got {t.device}")
-    if shape is not None and tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
-    if dtype is not None and t.dtype != dtype:
-        raise ValueError(f"{what}: expected dtype {dtype}, got {t.dtype}")
-    if contiguous and not t.is_contiguous():
-        raise ValueError(f"{what}: expected a contiguous tensor")
-    return t
+def _given(where, name, t, device, dtype, shape, contiguous=True):
+    """The address of `t` (None for None), which has to be on `device`, of this type and shape."""
+    if t is None:
+        return None
+    if t.get_device() == device and t.dtype is dtype and t.shape == shape and (not contiguous or t.is_contiguous()):
+        return t.data_ptr()
+    if t.get_device() != device:
+        raise ValueError(f"{where}: {name}: expected a tensor on the current CUDA device, got {t.device}")
+    if t.dtype is not dtype:
+        raise ValueError(f"{where}: {name}: expected dtype {dtype}, got {t.dtype}")
+    if t.shape != shape:
+        raise ValueError(f"{where}: {name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    raise ValueError(f"{where}: {name}: expected a contiguous tensor")
 
 
-def _rows_of(t, what):
+def _row_stride(where, name, t, rows, cols):
     """Row stride of a matrix whose rows are contiguous and do not overlap."""
-    rows, cols = t.shape
-    if (cols > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < cols):
-        raise ValueError(f"{what}: expected contiguous rows that do not overlap, got strides {t.stride()}")
-    return max(t.stride(0), cols) if rows > 1 else cols
+    if t.is_contiguous():
+        return cols
+    between, within = t.stride()
+    if (cols > 1 and within != 1) or (rows > 1 and between < cols):
+        raise ValueError(f"{where}: {name}: expected contiguous rows that do not overlap, got strides {t.stride()}")
+    return between if rows > 1 else cols
 
 
 def _distill_args(where, logits, teacher, index, teacher_lse, row_weight, temperature, scale):
-    import torch
-    if logits.dim() != 2 or index.dim() != 2 or index.shape[0] != logits.shape[0]:
+    device = _device_of(where, logits)
+    torch = _torch
+    if logits.dim() != 2 or index.dim() != 2:
         raise ValueError(f"{where}: expected logits [rows, vocab] and index [rows, k]")
     rows, vocab = logits.shape
-    _here(logits, f"{where}: logits", contiguous=False)
-    _here(index, f"{where}: index", dtype=torch.int64)
-    _here(teacher, f"{where}: teacher", index.shape)
-    if teacher_lse is not None:
-        _here(teacher_lse, f"{where}: teacher_lse", (rows,), torch.float32)
-    if row_weight is not None:
-        _here(row_weight, f"{where}: row_weight", (rows,), torch.float32)
-    if scale is None:
-        scale = 1.0 / max(rows, 1)
-    head = (_ptr(logits), _rows_of(logits, f"{where}: logits"), _dtype_code(logits, where), _ptr(teacher),
-            _dtype_code(teacher, where), _ptr(index), _ptr(teacher_lse), _ptr(row_weight))
-    return head, (rows, vocab, index.shape[1], temperature, scale)
+    k = index.shape[1]
+    row = (rows,)
+    head = (logits.data_ptr(), _row_stride(where, "logits", logits, rows, vocab), _dtype_code(where, logits),
+            _given(where, "teacher", teacher, device, teacher.dtype, (rows, k)), _dtype_code(where, teacher),
+            _given(where, "index", index, device, torch.int64, (rows, k)),
+            _given(where, "teacher_lse", teacher_lse, device, torch.float32, row),
+            _given(where, "row_weight", row_weight, device, torch.float32, row))
+    return device, head, (rows, vocab, k, temperature, 1.0 / max(rows, 1) if scale is None else scale)
 
 
-def _grad_for(where, logits, out):
-    import torch
+def _grad_for(where, logits, out, device):
+    rows, vocab = logits.shape
     if out is None:
-        return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device), logits.shape[1]
-    _here(out, f"{where}: out", logits.shape, logits.dtype, contiguous=False)
-    return out, _rows_of(out, f"{where}: out")
+        return _torch.empty((rows, vocab), dtype=logits.dtype, device=logits.device), vocab
+    _given(where, "out", out, device, logits.dtype, logits.shape, contiguous=False)
+    return out, _row_stride(where, "out", out, rows, vocab)
 
 
 def distill_topk(logits, teacher, index, teacher_lse=None, row_weight=None, temperature=1.0, scale=None):
@@ -427,28 +449,26 @@ def distill_topk(logits, teacher, index, teacher_lse=None, row_weight=None, temp
 
     logits [rows, vocab] (rows may be padded), teacher and index (int64) [rows, k]; an index outside
     [0, vocab) is padding.  scale: default 1 / rows (the mean).  row_stats goes to distill_topk_backward."""
-    import torch
-    head, sizes = _distill_args("distill_topk", logits, teacher, index, teacher_lse, row_weight, temperature, scale)
-    loss = torch.empty(1, dtype=torch.float32, device=logits.device)
-    row_loss = torch.empty(sizes[0], dtype=torch.float32, device=logits.device)
-    stats = torch.empty((sizes[0], 2), dtype=torch.float32, device=logits.device)
-    check(lib().fdl_distill_topk(*head, *sizes, _ptr(loss), _ptr(row_loss), _ptr(stats), _stream()), "fdl_distill_topk")
+    device, head, sizes = _distill_args("distill_topk", logits, teacher, index, teacher_lse, row_weight, temperature, scale)
+    rows, f32 = sizes[0], _torch.float32
+    loss = _torch.empty((1,), dtype=f32, device=logits.device)
+    row_loss = _torch.empty((rows,), dtype=f32, device=logits.device)
+    stats = _torch.empty((rows, 2), dtype=f32, device=logits.device)
+    check(lib().fdl_distill_topk(*head, *sizes, loss.data_ptr(), row_loss.data_ptr(), stats.data_ptr(),
+                                 _raw_stream(device)), "fdl_distill_topk")
     return loss, row_loss, stats
 
 
 def distill_topk_backward(logits, teacher, index, row_stats, teacher_lse=None, row_weight=None, temperature=1.0,
                           scale=None, grad_loss=None, out=None):
     """Gradient of grad_loss * loss in the logits' type; out may be `logits` itself."""
-    import torch
     where = "distill_topk_backward"
-    head, sizes = _distill_args(where, logits, teacher, index, teacher_lse, row_weight, temperature, scale)
-    _here(row_stats, f"{where}: row_stats", (sizes[0], 2), torch.float32)
-    if grad_loss is not None:
-        _here(grad_loss, f"{where}: grad_loss", dtype=torch.float32)
-        if grad_loss.numel() != 1:
-            raise ValueError(f"{where}: grad_loss: expected one value")
-    grad, stride = _grad_for(where, logits, out)
-    check(lib().fdl_distill_topk_backward(*head, _ptr(row_stats), _ptr(grad_loss), *sizes, _ptr(grad), stride, _stream()),
+    device, head, sizes = _distill_args(where, logits, teacher, index, teacher_lse, row_weight, temperature, scale)
+    f32 = _torch.float32
+    stats = _given(where, "row_stats", row_stats, device, f32, (sizes[0], 2))
+    up = None if grad_loss is None else _given(where, "grad_loss", grad_loss.reshape(-1), device, f32, (1,))
+    grad, stride = _grad_for(where, logits, out, device)
+    check(lib().fdl_distill_topk_backward(*head, stats, up, *sizes, grad.data_ptr(), stride, _raw_stream(device)),
           "fdl_distill_topk_backward")
     return grad
 
@@ -456,23 +476,16 @@ def distill_topk_backward(logits, teacher, index, row_stats, teacher_lse=None, r
 def distill_topk_with_grad(logits, teacher, index, teacher_lse=None, row_weight=None, temperature=1.0, scale=None,
                            out=None):
     """(loss [1], row_loss [rows], gradient of the loss); out may be `logits` itself."""
-    import torch
     where = "distill_topk_with_grad"
-    head, sizes = _distill_args(where, logits, teacher, index, teacher_lse, row_weight, temperature, scale)
-    loss = torch.empty(1, dtype=torch.float32, device=logits.device)
-    row_loss = torch.empty(sizes[0], dtype=torch.float32, device=logits.device)
-    stats = torch.empty((sizes[0], 2), dtype=torch.float32, device=logits.device)
-    grad, stride = _grad_for(where, logits, out)
-    check(lib().fdl_distill_topk_with_grad(*head, *sizes, _ptr(loss), _ptr(row_loss), _ptr(stats), _ptr(grad), stride,
-                                           _stream()), "fdl_distill_topk_with_grad")
+    device, head, sizes = _distill_args(where, logits, teacher, index, teacher_lse, row_weight, temperature, scale)
+    rows, f32 = sizes[0], _torch.float32
+    loss = _torch.empty((1,), dtype=f32, device=logits.device)
+    row_loss = _torch.empty((rows,), dtype=f32, device=logits.device)
+    stats = _torch.empty((rows, 2), dtype=f32, device=logits.device)
+    grad, stride = _grad_for(where, logits, out, device)
+    check(lib().fdl_distill_topk_with_grad(*head, *sizes, loss.data_ptr(), row_loss.data_ptr(), stats.data_ptr(),
+                                           grad.data_ptr(), stride, _raw_stream(device)), "fdl_distill_topk_with_grad")
     return loss, row_loss, grad
-
-
-def _norm_weights(where, cols, **weights):
-    import torch
-    for name, w in weights.items():
-        if w is not None:
-            _here(w, f"{where}: {name}", (cols,), torch.float32)
 
 
 def norm_residual(x, h, post=NORM_RMS, pre=NORM_RMS, gate=None, gate_act=GATE_PLAIN, post_gamma=None, post_beta=None,
@@ -480,27 +493,26 @@ def norm_residual(x, h, post=NORM_RMS, pre=NORM_RMS, gate=None, gate_act=GATE_PL
     """y = residual_scale * x + block_scale * act(gate) * norm_post(h) and n = norm_pre(y): (y, n, stats [rows, 4]).
 
     gate: [gate_rows, cols], gate_rows a divisor of rows.  n is None with pre=NORM_NONE.  out may be x, out_n h."""
-    import torch
     where = "norm_residual"
+    device = _device_of(where, x)
     if x.dim() != 2:
         raise ValueError(f"{where}: expected [rows, cols]")
-    rows, cols = x.shape
-    _here(x, f"{where}: x")
-    _here(h, f"{where}: h", (rows, cols), x.dtype)
-    gate_rows = 0
-    if gate is not None:
-        gate_rows = gate.shape[0]
-        _here(gate, f"{where}: gate", (gate_rows, cols), x.dtype)
-    _norm_weights(where, cols, post_gamma=post_gamma, post_beta=post_beta, pre_gamma=pre_gamma, pre_beta=pre_beta)
-    y = torch.empty_like(x) if out is None else _here(out, f"{where}: out", (rows, cols), x.dtype)
+    shape, kind, f32 = x.shape, x.dtype, _torch.float32
+    rows, cols = shape
+    col = (cols,)
+    gate_rows = 0 if gate is None else gate.shape[0]
+    y = _torch.empty_like(x) if out is None else out
     n = None
     if pre != NORM_NONE:
-        n = torch.empty_like(x) if out_n is None else _here(out_n, f"{where}: out_n", (rows, cols), x.dtype)
-    stats = torch.empty((rows, 4), dtype=torch.float32, device=x.device)
-    check(lib().fdl_norm_residual(_ptr(x), _ptr(h), _ptr(gate), gate_rows, gate_act, post, _ptr(post_gamma),
-                                  _ptr(post_beta), pre, _ptr(pre_gamma), _ptr(pre_beta), _ptr(y), _ptr(n), _ptr(stats),
-                                  rows, cols, residual_scale, block_scale, eps, _dtype_code(x, where), _stream()),
-          "fdl_norm_residual")
+        n = _torch.empty_like(x) if out_n is None else out_n
+    stats = _torch.empty((rows, 4), dtype=f32, device=x.device)
+    check(lib().fdl_norm_residual(
+        _given(where, "x", x, device, kind, shape), _given(where, "h", h, device, kind, shape),
+        _given(where, "gate", gate, device, kind, (gate_rows, cols)), gate_rows, gate_act, post,
+        _given(where, "post_gamma", post_gamma, device, f32, col), _given(where, "post_beta", post_beta, device, f32, col),
+        pre, _given(where, "pre_gamma", pre_gamma, device, f32, col), _given(where, "pre_beta", pre_beta, device, f32, col),
+        _given(where, "out", y, device, kind, shape), _given(where, "out_n", n, device, kind, shape), stats.data_ptr(),
+        rows, cols, residual_scale, block_scale, eps, _dtype_code(where, x), _raw_stream(device)), "fdl_norm_residual")
     return y, n, stats
 
 
@@ -509,37 +521,38 @@ def norm_residual_backward(dy, dn, y, h, stats, post=NORM_RMS, pre=NORM_RMS, gat
                            want_post_beta=False, want_pre_beta=False):
     """Gradients of norm_residual as a dict: x, h, gate, post_gamma, post_beta, pre_gamma, pre_beta (None where there
     is nothing to learn).  dy or dn may be None."""
-    import torch
     where = "norm_residual_backward"
+    device = _device_of(where, h)
     if h.dim() != 2:
         raise ValueError(f"{where}: expected [rows, cols]")
-    rows, cols = h.shape
-    _here(h, f"{where}: h")
-    for name, t in (("dy", dy), ("dn", dn), ("y", y)):
-        if t is not None:
-            _here(t, f"{where}: {name}", (rows, cols), h.dtype)
-    _here(stats, f"{where}: stats", (rows, 4), torch.float32)
-    gate_rows = 0
-    if gate is not None:
-        gate_rows = gate.shape[0]
-        _here(gate, f"{where}: gate", (gate_rows, cols), h.dtype)
-    _norm_weights(where, cols, post_gamma=post_gamma, post_beta=post_beta, pre_gamma=pre_gamma)
-    code = _dtype_code(h, where)
-
-    def sums(wanted):
-        return torch.empty(cols, dtype=torch.float32, device=h.device) if wanted else None
-
-    out = {"x": torch.empty_like(h), "h": torch.empty_like(h), "gate": None if gate is None else torch.empty_like(gate),
-           "post_gamma": sums(post_gamma is not None), "post_beta": sums(want_post_beta),
-           "pre_gamma": sums(pre_gamma is not None), "pre_beta": sums(want_pre_beta)}
+    shape, kind, f32 = h.shape, h.dtype, _torch.float32
+    rows, cols = shape
+    col = (cols,)
+    gate_rows = 0 if gate is None else gate.shape[0]
+    code = _dtype_code(where, h)
+    like, place = _torch.empty_like, h.device
     bytes_ = lib().fdl_norm_residual_backward_scratch_bytes(rows, cols, gate_rows)
-    scratch = torch.empty(bytes_, dtype=torch.uint8, device=h.device)
+    scratch = _torch.empty((bytes_,), dtype=_torch.uint8, device=place)
+    gx, gh, ggate = like(h), like(h), None if gate is None else like(gate)
+
+    def beta_sum(wanted, gamma):
+        if not wanted:
+            return None
+        return _torch.empty(col, dtype=f32, device=place) if gamma is None else like(gamma)
+
+    sums = (None if post_gamma is None else like(post_gamma), beta_sum(want_post_beta, post_gamma),
+            None if pre_gamma is None else like(pre_gamma), beta_sum(want_pre_beta, pre_gamma))
     check(lib().fdl_norm_residual_backward(
-        _ptr(dy), _ptr(dn), _ptr(y), _ptr(h), _ptr(stats), _ptr(gate), gate_rows, gate_act, post, _ptr(post_gamma),
-        _ptr(post_beta), pre, _ptr(pre_gamma), _ptr(out["x"]), _ptr(out["h"]), _ptr(out["gate"]), _ptr(out["post_gamma"]),
-        _ptr(out["post_beta"]), _ptr(out["pre_gamma"]), _ptr(out["pre_beta"]), rows, cols, residual_scale, block_scale,
-        code, _ptr(scratch), bytes_, _stream()), "fdl_norm_residual_backward")
-    return out
+        _given(where, "dy", dy, device, kind, shape), _given(where, "dn", dn, device, kind, shape),
+        _given(where, "y", y, device, kind, shape), _given(where, "h", h, device, kind, shape),
+        _given(where, "stats", stats, device, f32, (rows, 4)), _given(where, "gate", gate, device, kind, (gate_rows, cols)),
+        gate_rows, gate_act, post, _given(where, "post_gamma", post_gamma, device, f32, col),
+        _given(where, "post_beta", post_beta, device, f32, col), pre,
+        _given(where, "pre_gamma", pre_gamma, device, f32, col), gx.data_ptr(), gh.data_ptr(), _ptr(ggate), _ptr(sums[0]),
+        _ptr(sums[1]), _ptr(sums[2]), _ptr(sums[3]), rows, cols, residual_scale, block_scale, code, scratch.data_ptr(),
+        bytes_, _raw_stream(device)), "fdl_norm_residual_backward")
+    return {"x": gx, "h": gh, "gate": ggate, "post_gamma": sums[0], "post_beta": sums[1], "pre_gamma": sums[2],
+            "pre_beta": sums[3]}
 
 
 def verify_draft(target, draft_tokens, accept_u, sample_u, draft=None, draft_len=None):
@@ -547,31 +560,30 @@ def verify_draft(target, draft_tokens, accept_u, sample_u, draft=None, draft_len
 
     target [batch, drafted + 1, vocab], draft [batch, drafted, vocab] or None (a draft that is certain of its
     tokens), draft_tokens (int64) and accept_u [batch, drafted], sample_u [batch], draft_len (int64) [batch]."""
-    import torch
     where = "verify_draft"
     if target.dim() != 3 or draft_tokens.dim() != 2:
         raise ValueError(f"{where}: expected target [batch, drafted + 1, vocab] and draft_tokens [batch, drafted]")
+    device = _device_of(where, target)
+    kind, f32, i64 = target.dtype, _torch.float32, _torch.int64
     batch, drafted = draft_tokens.shape
     vocab = target.shape[2]
-    _here(target, f"{where}: target", (batch, drafted + 1, vocab), contiguous=False)
-    _here(draft_tokens, f"{where}: draft_tokens", dtype=torch.int64)
-    _here(accept_u, f"{where}: accept_u", (batch, drafted), torch.float32)
-    _here(sample_u, f"{where}: sample_u", (batch,), torch.float32)
-    if draft_len is not None:
-        _here(draft_len, f"{where}: draft_len", (batch,), torch.int64)
-    strides = [0, 0]
+    target_batch, target_row, within = target.stride()
+    draft_batch = draft_row = 0
     if draft is not None:
-        _here(draft, f"{where}: draft", (batch, drafted, vocab), target.dtype, contiguous=False)
-        strides = draft.stride()[:2]
-    for t in (target, draft):
-        if t is not None and vocab > 1 and t.stride(2) != 1:
-            raise ValueError(f"{where}: expected a contiguous last dimension, got strides {t.stride()}")
-    tokens = torch.empty((batch, drafted + 1), dtype=torch.int64, device=target.device)
-    accepted = torch.empty(batch, dtype=torch.int64, device=target.device)
-    check(lib().fdl_verify_draft(_ptr(target), target.stride(0), target.stride(1), _ptr(draft), strides[0], strides[1],
-                                 _dtype_code(target, where), _ptr(draft_tokens), _ptr(draft_len), _ptr(accept_u),
-                                 _ptr(sample_u), batch, drafted, vocab, _ptr(tokens), _ptr(accepted), _stream()),
-          "fdl_verify_draft")
+        draft_batch, draft_row, within_draft = draft.stride()
+        within = max(within, within_draft)
+    if vocab > 1 and within != 1:
+        raise ValueError(f"{where}: expected a contiguous last dimension")
+    tokens = _torch.empty((batch, drafted + 1), dtype=i64, device=target.device)
+    accepted = _torch.empty((batch,), dtype=i64, device=target.device)
+    check(lib().fdl_verify_draft(
+        _given(where, "target", target, device, kind, (batch, drafted + 1, vocab), contiguous=False), target_batch,
+        target_row, _given(where, "draft", draft, device, kind, (batch, drafted, vocab), contiguous=False), draft_batch,
+        draft_row, _dtype_code(where, target), _given(where, "draft_tokens", draft_tokens, device, i64, (batch, drafted)),
+        _given(where, "draft_len", draft_len, device, i64, (batch,)),
+        _given(where, "accept_u", accept_u, device, f32, (batch, drafted)),
+        _given(where, "sample_u", sample_u, device, f32, (batch,)), batch, drafted, vocab, tokens.data_ptr(),
+        accepted.data_ptr(), _raw_stream(device)), "fdl_verify_draft")
     return tokens, accepted
 
 
