@@ -19,8 +19,6 @@ namespace fdl {
 
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kWarps = kThreads / kWarp;
 constexpr int kMaxEntries = 1024;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -53,6 +51,7 @@ __device__ __forceinline__ float load_any(const void* p, int dtype, int64_t i) {
 // exp((a - b) / T) for a running maximum a <= b, with c = log2(e) / T; 1 when both are -inf.
 __device__ __forceinline__ float exp_diff(float a, float b, float c) { return a == b ? 1.0f : ex2_approx((a - b) * c); }
 
+template <int kWarps>
 __device__ __forceinline__ float block_max(float v, float* red) {
     v = warp_max(v);
     __syncthreads();
@@ -64,7 +63,7 @@ __device__ __forceinline__ float block_max(float v, float* red) {
     return v;
 }
 
-template <class S>
+template <int kWarps, class S>
 __device__ __forceinline__ S block_sum(S v, S* red) {
     v = warp_sum(v);
     __syncthreads();
@@ -88,10 +87,13 @@ struct RowSpan {
     }
 };
 
+// Short rows: a small CTA a row, many of them an SM, the row read a second time (out of L1 or L2) for its gradient.
+constexpr int kRowThreads = 128;
+
 template <class T, bool LOSS, bool GRAD>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kRowThreads)
 distill_rows_kernel(const DistillParams p) {
-    constexpr int N = kPack<T>;
+    constexpr int N = kPack<T>, kThreads = kRowThreads, kWarps = kThreads / kWarp;
     __shared__ float prob[kMaxEntries];
     __shared__ int at[kMaxEntries];
     __shared__ float here[kMaxEntries];
@@ -113,7 +115,7 @@ distill_rows_kernel(const DistillParams p) {
             at[j] = v > -INFINITY ? static_cast<int>(i) : -1;  // a NaN does not count either
             top = fmaxf(top, v);
         }
-        top = block_max(top, redf);
+        top = block_max<kWarps>(top, redf);
         const bool live = weight != 0.0f && top != -INFINITY;
         T* g = GRAD ? static_cast<T*>(p.grad) + row * p.grad_stride : nullptr;
         if (!live) {
@@ -135,7 +137,7 @@ distill_rows_kernel(const DistillParams p) {
                 part += ex2_approx((prob[j] - top) * c);
             }
         }
-        const float teacher_sum = block_sum(part, redf);
+        const float teacher_sum = block_sum<kWarps>(part, redf);
         const double log_norm = p.teacher_lse == nullptr
                                     ? static_cast<double>(top) * p.inv_temperature + log(static_cast<double>(teacher_sum))
                                     : static_cast<double>(p.teacher_lse[row]);
@@ -165,8 +167,8 @@ distill_rows_kernel(const DistillParams p) {
                 s = s * exp_diff(mx, now, c) + ex2_approx((v - (now == -INFINITY ? 0.0f : now)) * c);
                 mx = now;
             }
-            m = block_max(mx, redf);
-            total = block_sum(s * exp_diff(mx, m, c), redf);
+            m = block_max<kWarps>(mx, redf);
+            total = block_sum<kWarps>(s * exp_diff(mx, m, c), redf);
             if (t == 0) {
                 p.row_stats[2 * row] = m;
                 p.row_stats[2 * row + 1] = total;
@@ -190,11 +192,11 @@ distill_rows_kernel(const DistillParams p) {
             mass += pj;
         }
         if (LOSS) {
-            kl = block_sum(kl, redd);
+            kl = block_sum<kWarps>(kl, redd);
             if (t == 0) p.row_loss[row] = static_cast<float>(kl);
         }
         if (GRAD) {
-            mass = block_sum(mass, redf);
+            mass = block_sum<kWarps>(mass, redf);
             if (p.teacher_lse == nullptr) mass = mass == mass ? 1.0f : mass;
             float coef = p.scale * weight * static_cast<float>(p.inv_temperature);
             if (p.grad_loss != nullptr) coef *= *p.grad_loss;
@@ -231,6 +233,600 @@ distill_rows_kernel(const DistillParams p) {
     }
 }
 
+// ---- long rows: a ring of chunks in shared memory -----------------------------------------------------
+//
+// One CTA an SM, or a cluster of them a row, takes rows one after the other.  Four kinds of work run side
+// by side in it:
+//   warp 0   asks for the row's chunks (bulk-async copies) as places in the ring come free,
+//   warps 1-3  read the teacher's entries, each of every third row and so a few rows ahead: their
+//            probabilities, the student's logits there, entries that share a column folded into the first,
+//            what the loss needs of them (one warp for all rows was the slowest part of the kernel),
+//   the rest take a chunk of row i for its gradient, give its place back, and a chunk of row i + 1 for
+//            its maximum and sum of exponentials (each thread's own running pair; one exchange a row).
+// So a row is read once and its gradient written once, and the next row streams in while a row's gradient
+// streams out.  The loss alone and the gradient alone need no lag: a chunk is used and its place given back.
+// A chunk's places outside the 16-byte grid of the row (its first and last few elements) go by plain loads.
+//
+// Every wait has a limit; one that gives up ends all of them (and is reported through the error flag).
+
+constexpr int kChunkBytes = 16384;
+constexpr int kMaxSlots = 13;
+constexpr int kPrepSlots = 4;       // rows whose entries are kept
+constexpr int kPrepWarps = 3;       // 20 warps in all: one more would cost every thread 16 registers
+constexpr int kConsumerWarps = 16;  // two groups that take the chunks in turn
+constexpr int kConsumers = kConsumerWarps * kWarp;
+constexpr int kGroupWarps = kConsumerWarps / 2;
+constexpr int kGroup = kGroupWarps * kWarp;
+constexpr int kBatch = kChunkBytes / 16 / kGroup;  // packs of a chunk that a thread takes
+constexpr int kFirstConsumer = 1 + kPrepWarps;     // warp
+constexpr int kRingThreads = (kFirstConsumer + kConsumerWarps) * kWarp;
+constexpr int kMaxCluster = 8;
+constexpr int kRingSmem = 222 * 1024;  // of 227: the rest holds the static part
+
+struct Prepared {  // what is left of a row by its warp, beside the entries
+    double base;   // sum p_j (log p_j - logit_j / T)
+    double mass;
+    float weight, m, total;
+    int live;
+    float edge[16];
+};
+
+struct RingParams {
+    DistillParams d;
+    int slots;
+    int table;  // places of a hash table of columns, a power of two (one table for each prep warp)
+    unsigned int* error_flag;
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync_all() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+// Stores (m, s) into CTA `rank`'s copy of `mine`, counted as eight bytes on its copy of `bar`.  (An ordinary
+// store and a releasing arrival would wait for the warp's gradient stores, a microsecond or two a row.)
+__device__ __forceinline__ void send_stat(float2* mine, uint64_t* bar, uint32_t rank, float2 v) {
+    uint32_t to, at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_addr(mine)), "r"(rank));
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_addr(bar)), "r"(rank));
+    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(to), "f"(v.x),
+                 "f"(v.y), "r"(at)
+                 : "memory");
+}
+__device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(smem_addr(bar)), "r"(parity)
+        : "memory");
+    return done != 0;
+}
+
+// A wait that gives up raises `failed`, which ends every later wait of the CTA that is not over at once;
+// who gets false leaves.
+template <bool CLUSTER = false>
+__device__ __forceinline__ bool lane_wait(uint64_t* bar, uint32_t parity, volatile int* failed, unsigned int* error_flag) {
+    if (CLUSTER ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity)) return true;
+    for (uint32_t i = 0; i < kMbarSpinLimit; ++i) {
+        if (CLUSTER ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity)) return true;
+        if ((i & 15u) == 15u && *failed != 0) return false;
+    }
+    *failed = 1;
+    atomicOr_system(error_flag, 1u);
+    return false;
+}
+// The same for a whole warp, with one answer.
+template <bool CLUSTER = false>
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* failed, unsigned int* error_flag) {
+    return __all_sync(kFullMask, lane_wait<CLUSTER>(bar, parity, failed, error_flag));
+}
+
+// -inf in each element of a pack.
+__device__ __forceinline__ uint4 lowest_pack(float) { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
+__device__ __forceinline__ uint4 lowest_pack(__half) { return make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u); }
+__device__ __forceinline__ uint4 lowest_pack(__nv_bfloat16) { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
+
+// A position in a ring of `size` places: place and the parity of its round.
+struct RingPlace {
+    int place;
+    uint32_t parity;
+    __device__ __forceinline__ void next(int size) {
+        if (++place == size) {
+            place = 0;
+            parity ^= 1u;
+        }
+    }
+};
+
+// The part of a row that a CTA of the cluster owns: aligned packs [lo, hi), as chunks of `each` packs.
+template <class T>
+struct Slice {
+    RowSpan<T> span;
+    int lo, hi, chunks, each;
+    __device__ __forceinline__ Slice(const T* row, int vocab, int rank, int cluster) : span(row, vocab) {
+        lo = static_cast<int>(static_cast<int64_t>(span.packs) * rank / cluster);
+        hi = static_cast<int>(static_cast<int64_t>(span.packs) * (rank + 1) / cluster);
+        chunks = (hi - lo + kChunkBytes / 16 - 1) / (kChunkBytes / 16);
+        // equal chunks; of a very long row whole ones (so many equal ones could end before the last)
+        each = chunks > 256 ? kChunkBytes / 16 : chunks > 0 ? (hi - lo + chunks - 1) / chunks : 0;
+    }
+    __device__ __forceinline__ int begin(int c) const { return lo + c * each; }
+    __device__ __forceinline__ int size(int c) const { return min(each, hi - begin(c)); }
+    __device__ __forceinline__ int edges() const { return span.head + span.tail; }
+    __device__ __forceinline__ int edge_col(int i, int vocab) const { return i < span.head ? i : vocab - span.tail + (i - span.head); }
+    // Whether this CTA writes the gradient of `col` (rank 0 has the edges).
+    __device__ __forceinline__ bool owns(int col, int rank) const {
+        const int inner = col - span.head;
+        if (inner < 0 || inner >= span.packs * kPack<T>) return rank == 0;
+        const int pack = inner / kPack<T>;
+        return pack >= lo && pack < hi;
+    }
+};
+
+template <class T, bool LOSS, bool GRAD>
+__global__ void __launch_bounds__(kRingThreads, 1)
+distill_ring_kernel(const RingParams r) {
+    constexpr int N = kPack<T>;
+    constexpr bool kLag = LOSS && GRAD;
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ uint64_t full[kMaxSlots], empty[kMaxSlots], prep_full[kPrepSlots], prep_empty[kPrepSlots], stat_full[2];
+    __shared__ float2 stat[2][kMaxCluster * kConsumerWarps];
+    __shared__ Prepared prepared[kPrepSlots];
+    __shared__ int failed_word;
+    volatile int* const failed = &failed_word;
+    const DistillParams& p = r.d;
+    const int warp = threadIdx.x / kWarp, lane = threadIdx.x & (kWarp - 1);
+    const int rank = static_cast<int>(cluster_rank()), cluster = static_cast<int>(cluster_size());
+    const int64_t teams = gridDim.x / cluster, id = blockIdx.x / cluster;
+    const float c = static_cast<float>(kLog2e * p.inv_temperature);
+    unsigned char* const ring = smem;
+    float* const probs = reinterpret_cast<float*>(smem + static_cast<size_t>(r.slots) * kChunkBytes);  // [prep slots][k] each
+    float* const heres = probs + kPrepSlots * p.k;
+    int* const ats = reinterpret_cast<int*>(heres + kPrepSlots * p.k);
+    uint16_t* const tables = reinterpret_cast<uint16_t*>(ats + kPrepSlots * p.k);
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < r.slots; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], kGroupWarps);
+        }
+        for (int i = 0; i < kPrepSlots; ++i) {
+            mbar_init(&prep_full[i], 1);
+            mbar_init(&prep_empty[i], kConsumerWarps + 1);
+        }
+        for (int i = 0; i < 2; ++i) mbar_init(&stat_full[i], 1);
+        failed_word = 0;
+        fence_mbar_init();
+    }
+    __syncthreads();
+    if (cluster > 1) cluster_sync_all();  // every CTA's barriers are there before the first remote arrival
+    pdl_wait();
+
+    if (warp == 0) {
+        // ---- copies ----
+        if (lane == 0) {
+            RingPlace slot{0, 1}, prep{0, 0};  // the first round finds every place empty
+            int64_t asked = 0;
+            for (int64_t row = id; row < p.rows; row += teams) {
+                if (!lane_wait(&prep_full[prep.place], prep.parity, failed, r.error_flag)) break;
+                const bool live = prepared[prep.place].live != 0;
+                mbar_arrive(&prep_empty[prep.place]);
+                prep.next(kPrepSlots);
+                if (!live) continue;
+                const T* z = static_cast<const T*>(p.logits) + row * p.logits_stride;
+                const Slice<T> slice(z, p.vocab, rank, cluster);
+                const T* body = z + slice.span.head;
+                int i = 0;
+                for (; i < slice.chunks; ++i) {
+                    if (!lane_wait(&empty[slot.place], slot.parity, failed, r.error_flag)) break;
+                    const uint32_t bytes = static_cast<uint32_t>(slice.size(i)) * 16u;
+                    mbar_expect_tx(&full[slot.place], bytes);
+                    bulk_g2s(ring + static_cast<size_t>(slot.place) * kChunkBytes, body + static_cast<int64_t>(slice.begin(i)) * N,
+                             bytes, &full[slot.place]);
+                    slot.next(r.slots);
+                    ++asked;
+                }
+                if (i < slice.chunks) break;
+            }
+            if (*failed != 0) {  // copies that nobody waits for any more must not outlive the CTA
+                for (int64_t n = asked > r.slots ? asked - r.slots : 0; n < asked; ++n) {
+                    mbar_wait_bounded(&full[n % r.slots], static_cast<uint32_t>(n / r.slots) & 1u);
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp < kFirstConsumer) {
+        // ---- the teacher's entries ----
+        uint16_t* const table = tables + (warp - 1) * r.table;
+        for (int64_t number = warp - 1; id + number * teams < p.rows; number += kPrepWarps) {
+            const int64_t row = id + number * teams;
+            const int place = static_cast<int>(number % kPrepSlots);
+            // The first round finds the slots free.
+            if (!warp_wait(&prep_empty[place], static_cast<uint32_t>(number / kPrepSlots & 1) ^ 1u, failed, r.error_flag)) break;
+            float* const prob = probs + place * p.k;
+            float* const here = heres + place * p.k;
+            int* const at = ats + place * p.k;
+            Prepared& out = prepared[place];
+            const T* z = static_cast<const T*>(p.logits) + row * p.logits_stride;
+            const float weight = p.row_weight == nullptr ? 1.0f : p.row_weight[row];
+            float top = -INFINITY;
+            for (int j0 = lane; j0 < p.k; j0 += 4 * kWarp) {  // four entries' loads at a time
+                int64_t i[4];
+                float v[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int64_t from = row * p.k + min(j0 + q * kWarp, p.k - 1);
+                    i[q] = p.index[from];
+                    v[q] = load_any(p.teacher, p.teacher_dtype, from);
+                }
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int j = j0 + q * kWarp;
+                    if (j >= p.k) break;
+                    const bool counts = i[q] >= 0 && i[q] < p.vocab && v[q] > -INFINITY;  // a NaN does not either
+                    prob[j] = counts ? v[q] : -INFINITY;
+                    at[j] = counts ? static_cast<int>(i[q]) : -1;
+                    if (counts) top = fmaxf(top, v[q]);
+                }
+            }
+            top = warp_max(top);
+            const bool live = weight != 0.0f && top != -INFINITY;
+            if (live) {
+                const Slice<T> slice(z, p.vocab, rank, cluster);
+                float part = 0.0f;
+                for (int j0 = lane; j0 < p.k; j0 += 4 * kWarp) {
+                    float v[4];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int j = j0 + q * kWarp;
+                        const int col = j < p.k ? at[j] : -1;
+                        // (The gradient alone, in place: another CTA may be writing its part of the row already.)
+                        v[q] = col >= 0 && (LOSS || slice.owns(col, rank)) ? to_f32(z[col]) : 0.0f;
+                        if (col >= 0) part += ex2_approx((prob[j] - top) * c);
+                    }
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        if (j0 + q * kWarp < p.k) here[j0 + q * kWarp] = v[q];
+                    }
+                }
+                if (lane < slice.edges() && (LOSS || rank == 0)) out.edge[lane] = to_f32(z[slice.edge_col(lane, p.vocab)]);
+                const double sum = static_cast<double>(warp_sum(part));
+                const double norm = p.teacher_lse == nullptr ? static_cast<double>(top) * p.inv_temperature + log(sum)
+                                                             : static_cast<double>(p.teacher_lse[row]);
+                double base = 0.0, mass = 0.0;
+                for (int j = lane; j < p.k; j += kWarp) {
+                    float pj = 0.0f;
+                    if (at[j] >= 0) {
+                        const double logp = static_cast<double>(prob[j]) * p.inv_temperature - norm;
+                        pj = expf(static_cast<float>(logp));
+                        if (LOSS && pj != 0.0f) base += pj * (logp - static_cast<double>(here[j]) * p.inv_temperature);
+                        mass += pj;
+                    }
+                    prob[j] = pj;
+                }
+                base = warp_sum(base);
+                mass = warp_sum(mass);
+                if (GRAD) {
+                    // Entries of one column: each entry writes its number into the column's place of a hash table
+                    // and looks who is there.  Another column there: again with another hash (that column's own
+                    // entries are all in the same position); its own column: to be folded.  What the table held
+                    // before does not matter, as a place is read after at least one entry wrote it.
+                    uint32_t pending = 0, same = 0;  // bit q: entry lane + 32 q
+                    for (int j = lane, q = 0; j < p.k; j += kWarp, ++q) pending |= at[j] >= 0 ? 1u << q : 0u;
+                    for (uint32_t round = 0; __any_sync(kFullMask, pending != 0u); ++round) {
+                        const uint32_t mix = 0x9E3779B1u + 2u * round * 0x85EBCA6Bu;  // odd
+                        __syncwarp();
+                        for (uint32_t left = pending; left != 0u; left &= left - 1u) {
+                            const int j = lane + kWarp * (__ffs(left) - 1);
+                            table[(static_cast<uint32_t>(at[j] + 1) * mix >> 15) & (r.table - 1)] = static_cast<uint16_t>(j);
+                        }
+                        __syncwarp();
+                        for (uint32_t left = pending; left != 0u; left &= left - 1u) {
+                            const int q = __ffs(left) - 1, j = lane + kWarp * q;
+                            const int w = table[(static_cast<uint32_t>(at[j] + 1) * mix >> 15) & (r.table - 1)];
+                            if (w == j || at[w] == at[j]) {
+                                pending &= ~(1u << q);
+                                if (w != j) same |= 1u << q;
+                            }
+                        }
+                    }
+                    __syncwarp();
+                    // The first entry of a shared column gets the sum (in entry order over lanes, a fixed tree); the
+                    // others are dropped.
+                    for (uint32_t owners = __ballot_sync(kFullMask, same != 0u); owners != 0u;
+                         owners = __ballot_sync(kFullMask, same != 0u)) {
+                        const int owner = __ffs(owners) - 1;
+                        const int j = __shfl_sync(kFullMask, same != 0u ? lane + kWarp * (__ffs(same) - 1) : 0, owner);
+                        if (lane == owner) same &= same - 1u;
+                        const int col = at[j];
+                        if (col < 0) continue;  // dropped with an earlier one
+                        int least = p.k;
+                        float sum_p = 0.0f;
+                        for (int i = lane; i < p.k; i += kWarp) {
+                            if (at[i] == col) {
+                                least = min(least, i);
+                                sum_p += prob[i];
+                            }
+                        }
+                        least = __reduce_min_sync(kFullMask, least);
+                        sum_p = warp_sum(sum_p);
+                        __syncwarp();
+                        for (int i = lane; i < p.k; i += kWarp) {
+                            if (at[i] == col) {
+                                if (i == least) prob[i] = sum_p;
+                                else at[i] = -1;
+                            }
+                        }
+                        __syncwarp();
+                    }
+                }
+                if (lane == 0) {
+                    out.base = base;
+                    out.mass = mass;
+                    if (!LOSS) {
+                        out.m = p.row_stats[2 * row];
+                        out.total = p.row_stats[2 * row + 1];
+                    }
+                }
+            }
+            if (lane == 0) {
+                out.weight = weight;
+                out.live = live;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&prep_full[place]);
+        }
+    } else {
+        // ---- the logits ----
+        const int t = threadIdx.x - kFirstConsumer * kWarp, w = warp - kFirstConsumer;
+        const int group = w / kGroupWarps, tg = t % kGroup;
+        const float scale = p.scale * static_cast<float>(p.inv_temperature) *
+                            (GRAD && p.grad_loss != nullptr ? *p.grad_loss : 1.0f);
+        RingPlace slot{0, 0}, behind{0, 0};  // chunks of the current row, and of the row before (whose gradient lags)
+        RingPlace prep{0, 0}, prep_behind{0, 0};
+        uint32_t stat_round = 0;
+        struct Row {
+            int64_t row;
+            float m, total, coef;
+            float mass;
+        } cur{}, prev{};
+        bool has_prev = false;
+
+        auto release = [&](int place) {  // this warp is done with the place
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[place]);
+        };
+        auto write_chunk = [&](const Row& row, const Slice<T>& slice, int i, int place, T* g, bool same_phase) {
+            const unsigned char* chunk = ring + static_cast<size_t>(place) * kChunkBytes;
+            const float each = row.coef * row.mass / row.total;
+            const int n = slice.size(i);
+            T* out = g + slice.span.head + static_cast<int64_t>(slice.begin(i)) * N;
+            if (same_phase) {
+                uint4 raw[kBatch];
+#pragma unroll
+                for (int q = 0; q < kBatch; ++q) raw[q] = reinterpret_cast<const uint4*>(chunk)[tg + q * kGroup];
+                const float2 down = both(-row.m), c2 = both(c), each2 = both(each);
+                T* const mine = out + static_cast<int64_t>(tg) * N;
+#pragma unroll
+                for (int q = 0; q < kBatch; ++q) {
+                    if (tg + q * kGroup >= n) break;
+                    float2 v[N / 2];
+                    unpack2(raw[q], v, T{});
+#pragma unroll
+                    for (int e = 0; e < N / 2; ++e) {
+                        v[e] = mul2(add2(v[e], down), c2);
+                        v[e] = mul2(make_float2(ex2_approx(v[e].x), ex2_approx(v[e].y)), each2);
+                    }
+                    store_pairs(mine + q * kGroup * N, v);
+                }
+            } else {
+                for (int q = tg; q < n * N; q += kGroup) {
+                    out[q] = from_f32<T>(ex2_approx((to_f32(reinterpret_cast<const T*>(chunk)[q]) - row.m) * c) * each);
+                }
+            }
+        };
+        auto write_edges = [&](const Row& row, const Slice<T>& slice, const Prepared& pre, T* g) {
+            if (rank == 0 && t < slice.edges()) {
+                g[slice.edge_col(t, p.vocab)] = from_f32<T>(ex2_approx((pre.edge[t] - row.m) * c) * (row.coef * row.mass / row.total));
+            }
+        };
+        // The columns that the teacher names: each warp writes those of its own share of the row again, so
+        // that no barrier has to come between them and the dense part.
+        auto write_named = [&](const Row& row, const Slice<T>& slice, int place, T* g, bool same_phase) {
+            __syncwarp();
+            for (int j = lane; j < p.k; j += kWarp) {
+                const int col = ats[place * p.k + j];
+                if (col < 0 || !slice.owns(col, rank)) continue;
+                const int inner = col - slice.span.head;
+                int owner = 0;  // the edges: t < 16
+                if (inner >= 0 && inner < slice.span.packs * N) {
+                    const int pack = inner / N - slice.lo, chunk = pack / slice.each, in = pack - chunk * slice.each;
+                    const int thread = (same_phase ? in : in * N + inner % N) % kGroup;
+                    owner = (chunk & 1) * kGroupWarps + thread / kWarp;
+                }
+                if (owner != w) continue;
+                const float q = ex2_approx((heres[place * p.k + j] - row.m) * c) / row.total;
+                g[col] = from_f32<T>(row.coef * (row.mass * q - probs[place * p.k + j]));
+            }
+        };
+        auto phase_of = [&](const T* z, const T* g) {
+            return ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(g)) & 15) == 0;
+        };
+
+        for (int64_t at_row = id; at_row < p.rows || has_prev; at_row += teams) {
+            const bool has_cur = at_row < p.rows;
+            bool live = false;
+            if (has_cur) {
+                if (!warp_wait(&prep_full[prep.place], prep.parity, failed, r.error_flag)) break;
+                live = prepared[prep.place].live != 0;
+            }
+            const T* z = static_cast<const T*>(p.logits) + (has_cur ? at_row : id) * p.logits_stride;
+            const Slice<T> slice(z, p.vocab, rank, cluster);
+            const T* pz = static_cast<const T*>(p.logits) + (has_prev ? prev.row : id) * p.logits_stride;
+            T* pg = GRAD ? static_cast<T*>(p.grad) + (has_prev ? prev.row : id) * p.grad_stride : nullptr;
+            const Slice<T> pslice(pz, p.vocab, rank, cluster);
+            T* g = GRAD ? static_cast<T*>(p.grad) + (has_cur ? at_row : id) * p.grad_stride : nullptr;
+            cur.row = at_row;
+            if (live) {
+                cur.coef = scale * prepared[prep.place].weight;
+                cur.mass = p.teacher_lse == nullptr ? 1.0f : static_cast<float>(prepared[prep.place].mass);
+                if (prepared[prep.place].mass != prepared[prep.place].mass) cur.mass = NAN;
+                if (!LOSS) {
+                    cur.m = prepared[prep.place].m;
+                    cur.total = prepared[prep.place].total;
+                }
+            }
+            float mx = -INFINITY, s = 0.0f;
+            auto take_chunk = [&](const uint4* chunk, int n) {
+                uint4 raw[kBatch];
+#pragma unroll
+                for (int q = 0; q < kBatch; ++q) raw[q] = tg + q * kGroup < n ? chunk[tg + q * kGroup] : lowest_pack(T{});
+                float big = -INFINITY;
+#pragma unroll
+                for (int q = 0; q < kBatch; ++q) {
+                    float2 v[N / 2];
+                    unpack2(raw[q], v, T{});
+#pragma unroll
+                    for (int e = 0; e < N / 2; ++e) big = fmaxf(big, fmaxf(v[e].x, v[e].y));
+                }
+                const float now = fmaxf(mx, big);
+                const float ref = now == -INFINITY ? 0.0f : now;  // nothing but -inf so far: exp(-inf) each
+                const float2 down = both(-ref), c2 = both(c);
+                float2 add[2] = {both(0.0f), both(0.0f)};
+#pragma unroll
+                for (int q = 0; q < kBatch; ++q) {
+                    float2 v[N / 2];
+                    unpack2(raw[q], v, T{});
+#pragma unroll
+                    for (int e = 0; e < N / 2; ++e) {
+                        v[e] = mul2(add2(v[e], down), c2);
+                        add[e & 1] = add2(add[e & 1], make_float2(ex2_approx(v[e].x), ex2_approx(v[e].y)));
+                    }
+                }
+                const float2 sum = add2(add[0], add[1]);
+                s = s * exp_diff(mx, now, c) + (sum.x + sum.y);
+                mx = now;
+            };
+            const int steps = max(live ? slice.chunks : 0, kLag && has_prev ? pslice.chunks : 0);
+            const bool prev_phase = kLag && has_prev && phase_of(pz, pg), cur_phase = GRAD && phase_of(z, g);
+            bool ok = true;
+            for (int i = 0; i < steps; ++i) {
+                const bool mine = (i & 1) == group;  // the other group takes the other chunks
+                if (kLag && has_prev && i < pslice.chunks) {
+                    if (mine) {
+                        write_chunk(prev, pslice, i, behind.place, pg, prev_phase);
+                        release(behind.place);
+                    }
+                    behind.next(r.slots);
+                }
+                if (live && i < slice.chunks) {
+                    if (mine) {
+                        ok = warp_wait(&full[slot.place], slot.parity, failed, r.error_flag);
+                        if (!ok) break;
+                        if (LOSS) {
+                            take_chunk(reinterpret_cast<const uint4*>(ring + static_cast<size_t>(slot.place) * kChunkBytes), slice.size(i));
+                            if (!GRAD) release(slot.place);
+                        } else {
+                            write_chunk(cur, slice, i, slot.place, g, cur_phase);
+                            release(slot.place);
+                        }
+                    }
+                    slot.next(r.slots);
+                }
+            }
+            if (!ok) break;
+            if (kLag && has_prev) {
+                write_edges(prev, pslice, prepared[prep_behind.place], pg);
+                write_named(prev, pslice, prep_behind.place, pg, prev_phase);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&prep_empty[prep_behind.place]);
+                prep_behind.next(kPrepSlots);
+            }
+            if (live && LOSS) {
+                if (rank == 0 && w == 0) {
+                    const bool is_edge = lane < slice.edges();
+                    const float v = is_edge ? prepared[prep.place].edge[lane] : -INFINITY;
+                    const float now = fmaxf(mx, v);
+                    s = s * exp_diff(mx, now, c) + (is_edge ? ex2_approx((v - (now == -INFINITY ? 0.0f : now)) * c) : 0.0f);
+                    mx = now;
+                }
+                const float top = warp_max(mx);
+                const float2 mine = make_float2(top, warp_sum(s * exp_diff(mx, top, c)));
+                const int half = static_cast<int>(stat_round & 1u);
+                if (t == 0) mbar_expect_tx(&stat_full[half], static_cast<uint32_t>(cluster * kConsumerWarps * sizeof(float2)));
+                if (lane < cluster) send_stat(&stat[half][rank * kConsumerWarps + w], &stat_full[half], lane, mine);
+                if (!warp_wait<true>(&stat_full[half], (stat_round >> 1) & 1u, failed, r.error_flag)) break;
+                ++stat_round;
+                const int n = cluster * kConsumerWarps;
+                float m = -INFINITY;
+                for (int i = lane; i < n; i += kWarp) m = fmaxf(m, stat[half][i].x);
+                m = warp_max(m);
+                float sum = 0.0f;
+                for (int i = lane; i < n; i += kWarp) sum += stat[half][i].y * exp_diff(stat[half][i].x, m, c);
+                sum = warp_sum(sum);
+                cur.m = m;
+                cur.total = sum;
+                if (rank == 0 && t == 0) {
+                    p.row_stats[2 * at_row] = m;
+                    p.row_stats[2 * at_row + 1] = sum;
+                    const Prepared& pre = prepared[prep.place];
+                    p.row_loss[at_row] = static_cast<float>(
+                        pre.base + pre.mass * (static_cast<double>(m) * p.inv_temperature + log(static_cast<double>(sum))));
+                }
+            }
+            if (has_cur && !live) {  // left out
+                if (LOSS && rank == 0 && t == 0) {
+                    p.row_stats[2 * at_row] = 0.0f;
+                    p.row_stats[2 * at_row + 1] = 0.0f;
+                    p.row_loss[at_row] = 0.0f;
+                }
+                if (GRAD) {
+                    T* out = g + slice.span.head + static_cast<int64_t>(slice.lo) * N;
+                    const int n = slice.hi - slice.lo;
+                    if (cur_phase) {
+                        for (int q = t; q < n; q += kConsumers) __stcs(reinterpret_cast<uint4*>(out) + q, make_uint4(0, 0, 0, 0));
+                    } else {
+                        for (int q = t; q < n * N; q += kConsumers) out[q] = from_f32<T>(0.0f);
+                    }
+                    if (rank == 0 && t < slice.edges()) g[slice.edge_col(t, p.vocab)] = from_f32<T>(0.0f);
+                }
+            }
+            if (!LOSS && live) {
+                write_edges(cur, slice, prepared[prep.place], g);
+                write_named(cur, slice, prep.place, g, cur_phase);
+            }
+            if (has_cur) {
+                has_prev = kLag && live;
+                if (has_prev) {
+                    prev = cur;
+                    prep_behind = prep;
+                } else {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&prep_empty[prep.place]);
+                }
+                prep.next(kPrepSlots);
+            } else {
+                has_prev = false;
+            }
+        }
+    }
+    __syncthreads();
+    if (cluster > 1) cluster_sync_all();  // no CTA leaves while another may still send to it
+}
+
 // loss = scale * sum of weight * row loss, in 64 bits and in a fixed order.
 __global__ void __launch_bounds__(1024)
 distill_mean_kernel(const float* row_loss, const float* row_weight, int64_t rows, float scale, float* loss) {
@@ -261,15 +857,90 @@ int check_common(const void* logits, int64_t stride, int dtype, const void* teac
     return FDL_OK;
 }
 
+// Clusters of `cluster` ring CTAs that fit the device at once (asked once for each kernel, size and device).
+template <class K>
+int active_clusters(K kernel, int* cache, const DeviceInfo* info, int cluster, size_t smem, int* out) {
+    if (cluster == 1) {
+        *out = info->sm_count;
+        return FDL_OK;
+    }
+    int log2 = 0;
+    while ((1 << log2) < cluster) ++log2;
+    int& known = cache[(info->device % kMaxDevicesTracked) * 4 + log2];
+    if (known == 0) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(static_cast<unsigned int>(info->sm_count / cluster * cluster));
+        cfg.blockDim = dim3(kRingThreads);
+        cfg.dynamicSmemBytes = smem;
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = static_cast<unsigned int>(cluster);
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        int n = 0;
+        const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
+        if (e != cudaSuccess) return static_cast<int>(e);
+        known = n < 1 ? 1 : n;
+    }
+    *out = known;
+    return FDL_OK;
+}
+
+template <class T, bool LOSS, bool GRAD>
+int launch_ring(const DistillParams& p, const DeviceInfo* info, int cluster, int slots, int table, cudaStream_t stream) {
+    static int cache[kMaxDevicesTracked * 4] = {};
+    auto kernel = distill_ring_kernel<T, LOSS, GRAD>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    int most = 0;
+    int status = active_clusters(kernel, cache, info, cluster, kRingSmem, &most);
+    if (status != FDL_OK) return status;
+    RingParams r{p, slots, table, nullptr};
+    status = error_flag_device_ptr(&r.error_flag);
+    if (status != FDL_OK) return status;
+    const int64_t teams = p.rows < most ? p.rows : most;
+    return launch_ex(kernel, dim3(static_cast<unsigned int>(teams * cluster)), dim3(kRingThreads), kRingSmem, stream,
+                     dim3(static_cast<unsigned int>(cluster), 1, 1), tuning().pdl != 0, r);
+}
+
+// Rows of at least this many bytes take the ring form.
+constexpr int64_t kRingFromBytes = 16384;
+
 template <bool LOSS, bool GRAD>
 int launch_rows(const DistillParams& p, int dtype, cudaStream_t stream) {
     int status = FDL_OK;
     const DeviceInfo* info = current_device_info(&status);
     if (info == nullptr) return status;
-    const int grid = persistent_grid(info, 4, p.rows);
+    const int64_t bytes = static_cast<int64_t>(p.vocab) * static_cast<int64_t>(dtype_bytes(dtype));
+    if (bytes >= kRingFromBytes) {
+        int table = 64;
+        while (table < 2 * p.k) table *= 2;
+        const int64_t entries = static_cast<int64_t>(kPrepSlots) * p.k * 12 + kPrepWarps * 2 * table;
+        int64_t slots = (kRingSmem - entries) / kChunkBytes;
+        if (slots > kMaxSlots) slots = kMaxSlots;
+        // Loss and gradient together: a CTA's part of the row stays in the ring, with three chunks of the next.
+        int cluster = 1;
+        auto chunks = [&]() { return ceil_div(ceil_div(bytes, cluster), kChunkBytes) + 1; };
+        while (LOSS && GRAD && cluster < kMaxCluster && chunks() + 3 > slots) cluster *= 2;
+        // Fewer rows than SMs: more CTAs a row, down to a chunk each.
+        while (cluster < kMaxCluster && p.rows * cluster * 2 <= info->sm_count && bytes > static_cast<int64_t>(cluster) * kChunkBytes) {
+            cluster *= 2;
+        }
+        if (!(LOSS && GRAD) || chunks() + 1 <= slots) {
+            return with_dtype(dtype, [&](auto* tag) {
+                using T = std::remove_pointer_t<decltype(tag)>;
+                return launch_ring<T, LOSS, GRAD>(p, info, cluster, static_cast<int>(slots), table, stream);
+            });
+        }
+        // Longer than a cluster's shared memory: the loss, then the gradient from its statistics.
+        status = launch_rows<true, false>(p, dtype, stream);
+        return status != FDL_OK ? status : launch_rows<false, true>(p, dtype, stream);
+    }
+    const int grid = persistent_grid(info, 16, p.rows);
     return with_dtype(dtype, [&](auto* tag) {
         using T = std::remove_pointer_t<decltype(tag)>;
-        return launch_ex(distill_rows_kernel<T, LOSS, GRAD>, dim3(grid), dim3(kThreads), 0, stream, dim3(1, 1, 1),
+        return launch_ex(distill_rows_kernel<T, LOSS, GRAD>, dim3(grid), dim3(kRowThreads), 0, stream, dim3(1, 1, 1),
                          tuning().pdl != 0, p);
     });
 }

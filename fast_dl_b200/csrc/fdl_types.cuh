@@ -95,6 +95,59 @@ struct Chunk<T, 1> {
     __device__ static __forceinline__ void store_stream(T* p, const float (&v)[1]) { __stcs(p, from_f32<T>(v[0])); }
 };
 
+// Two floats in one instruction (a rounding each, as for one).
+__device__ __forceinline__ uint64_t bits2(float2 v) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y));
+    return r;
+}
+__device__ __forceinline__ float2 floats2(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)), "l"(bits2(c)));
+    return floats2(d);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)));
+    return floats2(d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)));
+    return floats2(d);
+}
+
+// A 128-bit pack as pairs.
+__device__ __forceinline__ void unpack2(const uint4& u, float2 (&v)[2], float) {
+    v[0] = make_float2(__uint_as_float(u.x), __uint_as_float(u.y));
+    v[1] = make_float2(__uint_as_float(u.z), __uint_as_float(u.w));
+}
+__device__ __forceinline__ void unpack2(const uint4& u, float2 (&v)[4], __half) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+}
+__device__ __forceinline__ void unpack2(const uint4& u, float2 (&v)[4], __nv_bfloat16) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+}
+template <class T, int M>
+__device__ __forceinline__ void store_pairs(T* p, const float2 (&v)[M]) {
+    float f[2 * M];
+#pragma unroll
+    for (int e = 0; e < M; ++e) {
+        f[2 * e] = v[e].x;
+        f[2 * e + 1] = v[e].y;
+    }
+    __stcs(reinterpret_cast<uint4*>(p), repack(f, T{}));
+}
 // 2^x with a relative error of about 2^-22.
 __device__ __forceinline__ float ex2_approx(float x) {
     float y;
