@@ -352,27 +352,31 @@ struct RingPlace {
     }
 };
 
-// The part of a row that a CTA of the cluster owns: aligned packs [lo, hi), as chunks of `each` packs.
+// The part of a row that a CTA of the cluster owns: aligned packs [lo, hi), in chunks of kChunkPacks.
+constexpr int kChunkPacks = kChunkBytes / 16;
 template <class T>
 struct Slice {
-    RowSpan<T> span;
-    int lo, hi, chunks, each;
-    __device__ __forceinline__ Slice(const T* row, int vocab, int rank, int cluster) : span(row, vocab) {
-        lo = static_cast<int>(static_cast<int64_t>(span.packs) * rank / cluster);
-        hi = static_cast<int>(static_cast<int64_t>(span.packs) * (rank + 1) / cluster);
-        chunks = (hi - lo + kChunkBytes / 16 - 1) / (kChunkBytes / 16);
-        // equal chunks; of a very long row whole ones (so many equal ones could end before the last)
-        each = chunks > 256 ? kChunkBytes / 16 : chunks > 0 ? (hi - lo + chunks - 1) / chunks : 0;
+    int head, tail, lo, hi;  // (the edges are in elements)
+    int packs, chunks;
+    __device__ __forceinline__ Slice(const T* row, int vocab, int rank, int log2_cluster) {
+        const RowSpan<T> span(row, vocab);
+        head = span.head;
+        tail = span.tail;
+        packs = span.packs;
+        lo = static_cast<int>(static_cast<int64_t>(packs) * rank >> log2_cluster);
+        hi = static_cast<int>(static_cast<int64_t>(packs) * (rank + 1) >> log2_cluster);
+        chunks = (hi - lo + kChunkPacks - 1) / kChunkPacks;
     }
-    __device__ __forceinline__ int begin(int c) const { return lo + c * each; }
-    __device__ __forceinline__ int size(int c) const { return min(each, hi - begin(c)); }
-    __device__ __forceinline__ int edges() const { return span.head + span.tail; }
-    __device__ __forceinline__ int edge_col(int i, int vocab) const { return i < span.head ? i : vocab - span.tail + (i - span.head); }
+    __device__ __forceinline__ int begin(int c) const { return lo + c * kChunkPacks; }
+    __device__ __forceinline__ int size(int c) const { return min(kChunkPacks, hi - begin(c)); }
+    __device__ __forceinline__ int edges() const { return head + tail; }
+    __device__ __forceinline__ int edge_col(int i, int vocab) const { return i < head ? i : vocab - tail + (i - head); }
+    // Whether `col` is one of the aligned packs.
+    __device__ __forceinline__ bool inner(int col) const { return static_cast<unsigned>(col - head) < static_cast<unsigned>(packs) * kPack<T>; }
     // Whether this CTA writes the gradient of `col` (rank 0 has the edges).
     __device__ __forceinline__ bool owns(int col, int rank) const {
-        const int inner = col - span.head;
-        if (inner < 0 || inner >= span.packs * kPack<T>) return rank == 0;
-        const int pack = inner / kPack<T>;
+        if (!inner(col)) return rank == 0;
+        const int pack = (col - head) / kPack<T>;
         return pack >= lo && pack < hi;
     }
 };
@@ -392,6 +396,7 @@ distill_ring_kernel(const RingParams r) {
     const int warp = threadIdx.x / kWarp, lane = threadIdx.x & (kWarp - 1);
     const int rank = static_cast<int>(cluster_rank()), cluster = static_cast<int>(cluster_size());
     const int64_t teams = gridDim.x / cluster, id = blockIdx.x / cluster;
+    const int log2_cluster = 31 - __clz(cluster);
     const float c = static_cast<float>(kLog2e * p.inv_temperature);
     unsigned char* const ring = smem;
     float* const probs = reinterpret_cast<float*>(smem + static_cast<size_t>(r.slots) * kChunkBytes);  // [prep slots][k] each
@@ -427,8 +432,8 @@ distill_ring_kernel(const RingParams r) {
                 prep.next(kPrepSlots);
                 if (!live) continue;
                 const T* z = static_cast<const T*>(p.logits) + row * p.logits_stride;
-                const Slice<T> slice(z, p.vocab, rank, cluster);
-                const T* body = z + slice.span.head;
+                const Slice<T> slice(z, p.vocab, rank, log2_cluster);
+                const T* body = z + slice.head;
                 int i = 0;
                 for (; i < slice.chunks; ++i) {
                     if (!lane_wait(&empty[slot.place], slot.parity, failed, r.error_flag)) break;
@@ -485,7 +490,7 @@ distill_ring_kernel(const RingParams r) {
             top = warp_max(top);
             const bool live = weight != 0.0f && top != -INFINITY;
             if (live) {
-                const Slice<T> slice(z, p.vocab, rank, cluster);
+                const Slice<T> slice(z, p.vocab, rank, log2_cluster);
                 float part = 0.0f;
                 for (int j0 = lane; j0 < p.k; j0 += 4 * kWarp) {
                     float v[4];
@@ -603,7 +608,9 @@ distill_ring_kernel(const RingParams r) {
             float m, total, coef;
             float mass;
         } cur{}, prev{};
-        bool has_prev = false;
+        bool has_prev = false, prev_phase = false;
+        T* pg = nullptr;
+        Slice<T> pslice(static_cast<const T*>(p.logits), p.vocab, rank, log2_cluster);
 
         auto release = [&](int place) {  // this warp is done with the place
             __syncwarp();
@@ -613,7 +620,7 @@ distill_ring_kernel(const RingParams r) {
             const unsigned char* chunk = ring + static_cast<size_t>(place) * kChunkBytes;
             const float each = row.coef * row.mass / row.total;
             const int n = slice.size(i);
-            T* out = g + slice.span.head + static_cast<int64_t>(slice.begin(i)) * N;
+            T* out = g + slice.head + static_cast<int64_t>(slice.begin(i)) * N;
             if (same_phase) {
                 uint4 raw[kBatch];
 #pragma unroll
@@ -650,12 +657,11 @@ distill_ring_kernel(const RingParams r) {
             for (int j = lane; j < p.k; j += kWarp) {
                 const int col = ats[place * p.k + j];
                 if (col < 0 || !slice.owns(col, rank)) continue;
-                const int inner = col - slice.span.head;
                 int owner = 0;  // the edges: t < 16
-                if (inner >= 0 && inner < slice.span.packs * N) {
-                    const int pack = inner / N - slice.lo, chunk = pack / slice.each, in = pack - chunk * slice.each;
-                    const int thread = (same_phase ? in : in * N + inner % N) % kGroup;
-                    owner = (chunk & 1) * kGroupWarps + thread / kWarp;
+                if (slice.inner(col)) {
+                    const int pack = (col - slice.head) / N - slice.lo, in = pack % kChunkPacks;
+                    const int thread = (same_phase ? in : in * N + (col - slice.head) % N) % kGroup;
+                    owner = (pack / kChunkPacks % 2) * kGroupWarps + thread / kWarp;
                 }
                 if (owner != w) continue;
                 const float q = ex2_approx((heres[place * p.k + j] - row.m) * c) / row.total;
@@ -674,10 +680,7 @@ distill_ring_kernel(const RingParams r) {
                 live = prepared[prep.place].live != 0;
             }
             const T* z = static_cast<const T*>(p.logits) + (has_cur ? at_row : id) * p.logits_stride;
-            const Slice<T> slice(z, p.vocab, rank, cluster);
-            const T* pz = static_cast<const T*>(p.logits) + (has_prev ? prev.row : id) * p.logits_stride;
-            T* pg = GRAD ? static_cast<T*>(p.grad) + (has_prev ? prev.row : id) * p.grad_stride : nullptr;
-            const Slice<T> pslice(pz, p.vocab, rank, cluster);
+            const Slice<T> slice(z, p.vocab, rank, log2_cluster);
             T* g = GRAD ? static_cast<T*>(p.grad) + (has_cur ? at_row : id) * p.grad_stride : nullptr;
             cur.row = at_row;
             if (live) {
@@ -721,7 +724,7 @@ distill_ring_kernel(const RingParams r) {
                 mx = now;
             };
             const int steps = max(live ? slice.chunks : 0, kLag && has_prev ? pslice.chunks : 0);
-            const bool prev_phase = kLag && has_prev && phase_of(pz, pg), cur_phase = GRAD && phase_of(z, g);
+            const bool cur_phase = GRAD && phase_of(z, g);
             bool ok = true;
             for (int i = 0; i < steps; ++i) {
                 const bool mine = (i & 1) == group;  // the other group takes the other chunks
@@ -748,13 +751,6 @@ distill_ring_kernel(const RingParams r) {
                 }
             }
             if (!ok) break;
-            if (kLag && has_prev) {
-                write_edges(prev, pslice, prepared[prep_behind.place], pg);
-                write_named(prev, pslice, prep_behind.place, pg, prev_phase);
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&prep_empty[prep_behind.place]);
-                prep_behind.next(kPrepSlots);
-            }
             if (live && LOSS) {
                 if (rank == 0 && w == 0) {
                     const bool is_edge = lane < slice.edges();
@@ -768,6 +764,16 @@ distill_ring_kernel(const RingParams r) {
                 const int half = static_cast<int>(stat_round & 1u);
                 if (t == 0) mbar_expect_tx(&stat_full[half], static_cast<uint32_t>(cluster * kConsumerWarps * sizeof(float2)));
                 if (lane < cluster) send_stat(&stat[half][rank * kConsumerWarps + w], &stat_full[half], lane, mine);
+            }
+            if (kLag && has_prev) {  // while the sums travel
+                write_edges(prev, pslice, prepared[prep_behind.place], pg);
+                write_named(prev, pslice, prep_behind.place, pg, prev_phase);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&prep_empty[prep_behind.place]);
+                prep_behind.next(kPrepSlots);
+            }
+            if (live && LOSS) {
+                const int half = static_cast<int>(stat_round & 1u);
                 if (!warp_wait<true>(&stat_full[half], (stat_round >> 1) & 1u, failed, r.error_flag)) break;
                 ++stat_round;
                 const int n = cluster * kConsumerWarps;
@@ -794,7 +800,7 @@ distill_ring_kernel(const RingParams r) {
                     p.row_loss[at_row] = 0.0f;
                 }
                 if (GRAD) {
-                    T* out = g + slice.span.head + static_cast<int64_t>(slice.lo) * N;
+                    T* out = g + slice.head + static_cast<int64_t>(slice.lo) * N;
                     const int n = slice.hi - slice.lo;
                     if (cur_phase) {
                         for (int q = t; q < n; q += kConsumers) __stcs(reinterpret_cast<uint4*>(out) + q, make_uint4(0, 0, 0, 0));
@@ -813,6 +819,9 @@ distill_ring_kernel(const RingParams r) {
                 if (has_prev) {
                     prev = cur;
                     prep_behind = prep;
+                    pslice = slice;
+                    pg = g;
+                    prev_phase = cur_phase;
                 } else {
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&prep_empty[prep.place]);
