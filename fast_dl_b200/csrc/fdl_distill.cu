@@ -235,33 +235,37 @@ distill_rows_kernel(const DistillParams p) {
 
 // ---- long rows: a ring of chunks in shared memory -----------------------------------------------------
 //
-// One CTA an SM, or a cluster of them a row, takes rows one after the other.  Four kinds of work run side
-// by side in it:
-//   warp 0   asks for the row's chunks (bulk-async copies) as places in the ring come free,
-//   warps 1-3  read the teacher's entries, each of every third row and so a few rows ahead: their
+// One CTA an SM, or a cluster of them a row, takes rows one after the other.  Its warps have trades, and each
+// goes on as soon as what it needs is there:
+//   copies   one thread asks for the row's chunks (bulk-async copies) as places in the ring come free;
+//   entries  three warps read the teacher's entries, each of every third row and so a few rows ahead: their
 //            probabilities, the student's logits there, entries that share a column folded into the first,
-//            what the loss needs of them (one warp for all rows was the slowest part of the kernel),
-//   the rest take a chunk of row i for its gradient, give its place back, and a chunk of row i + 1 for
-//            its maximum and sum of exponentials (each thread's own running pair; one exchange a row).
-// So a row is read once and its gradient written once, and the next row streams in while a row's gradient
-// streams out.  The loss alone and the gradient alone need no lag: a chunk is used and its place given back.
-// A chunk's places outside the 16-byte grid of the row (its first and last few elements) go by plain loads.
+//            what the loss needs of them (one warp for all rows was the slowest part of the kernel);
+//   sums     eight warps take each chunk for the row's maximum and sum of exponentials, every thread with a
+//            running pair of its own, and send each warp's pair to all CTAs of the cluster;
+//   writes   eight warps wait for the pairs, fold them, write the gradient chunk by chunk and give the places back.
+// So a row is read once and its gradient written once; the sums of row i + 1 are under way while the gradient of
+// row i is written, and the exchange between them falls to nobody's wait as long as the ring holds more than
+// the row.  The loss alone has two groups of eight warps for the sums, which take the chunks in turn, the
+// gradient alone two groups for the writes.
+// The elements of a row outside its 16-byte grid (its first and last few) go by plain loads.
 //
 // Every wait has a limit; one that gives up ends all of them (and is reported through the error flag).
 
 constexpr int kChunkBytes = 16384;
 constexpr int kMaxSlots = 13;
-constexpr int kPrepSlots = 4;       // rows whose entries are kept
-constexpr int kPrepWarps = 3;       // 20 warps in all: one more would cost every thread 16 registers
-constexpr int kConsumerWarps = 16;  // two groups that take the chunks in turn
-constexpr int kConsumers = kConsumerWarps * kWarp;
-constexpr int kGroupWarps = kConsumerWarps / 2;
+constexpr int kPrepSlots = 4;   // rows whose entries are kept
+constexpr int kPrepWarps = 3;   // 20 warps in all: one more would cost every thread 16 registers
+constexpr int kGroupWarps = 8;  // a group takes a whole chunk
 constexpr int kGroup = kGroupWarps * kWarp;
 constexpr int kBatch = kChunkBytes / 16 / kGroup;  // packs of a chunk that a thread takes
-constexpr int kFirstConsumer = 1 + kPrepWarps;     // warp
-constexpr int kRingThreads = (kFirstConsumer + kConsumerWarps) * kWarp;
+constexpr int kFirstWorker = 1 + kPrepWarps;       // warp
+constexpr int kRingThreads = (kFirstWorker + 2 * kGroupWarps) * kWarp;
 constexpr int kMaxCluster = 8;
-constexpr int kRingSmem = 222 * 1024;  // of 227: the rest holds the static part
+// Rows whose pairs may be on their way: a CTA whose writes have not read those of row i keeps its entries' slot,
+// so its sums end at row i + 3, the other CTAs' writes too, and their sums at row i + 7.
+constexpr int kStatSlots = 2 * kPrepSlots;
+constexpr int kRingSmem = 216 * 1024;  // of 227: the rest holds the static part
 
 struct Prepared {  // what is left of a row by its warp, beside the entries
     double base;   // sum p_j (log p_j - logit_j / T)
@@ -381,14 +385,37 @@ struct Slice {
     }
 };
 
+// The row's maximum and sum from the warps' pairs: the same order, and so the same bits, in every warp and CTA.
+__device__ __forceinline__ float2 fold_stats(const float2* stat, int n, float c) {
+    const int lane = threadIdx.x & (kWarp - 1);
+    float m = -INFINITY;
+    for (int i = lane; i < n; i += kWarp) m = fmaxf(m, stat[i].x);
+    m = warp_max(m);
+    float sum = 0.0f;
+    for (int i = lane; i < n; i += kWarp) sum += stat[i].y * exp_diff(stat[i].x, m, c);
+    return make_float2(m, warp_sum(sum));
+}
+__device__ __forceinline__ void write_loss(const DistillParams& p, const Prepared& pre, int64_t row, float2 f) {
+    p.row_stats[2 * row] = f.x;
+    p.row_stats[2 * row + 1] = f.y;
+    p.row_loss[row] = static_cast<float>(
+        pre.base + pre.mass * (static_cast<double>(f.x) * p.inv_temperature + log(static_cast<double>(f.y))));
+}
+__device__ __forceinline__ void write_left_out(const DistillParams& p, int64_t row) {
+    p.row_stats[2 * row] = 0.0f;
+    p.row_stats[2 * row + 1] = 0.0f;
+    p.row_loss[row] = 0.0f;
+}
+
 template <class T, bool LOSS, bool GRAD>
 __global__ void __launch_bounds__(kRingThreads, 1)
 distill_ring_kernel(const RingParams r) {
     constexpr int N = kPack<T>;
-    constexpr bool kLag = LOSS && GRAD;
+    constexpr int kSumGroups = !LOSS ? 0 : GRAD ? 1 : 2, kWriteGroups = !GRAD ? 0 : LOSS ? 1 : 2;
+    constexpr int kSumWarps = kSumGroups * kGroupWarps;
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ uint64_t full[kMaxSlots], empty[kMaxSlots], prep_full[kPrepSlots], prep_empty[kPrepSlots], stat_full[2];
-    __shared__ float2 stat[2][kMaxCluster * kConsumerWarps];
+    __shared__ uint64_t full[kMaxSlots], empty[kMaxSlots], prep_full[kPrepSlots], prep_empty[kPrepSlots], stat_full[kStatSlots];
+    __shared__ float2 stat[LOSS ? kStatSlots : 1][kMaxCluster * (GRAD ? 1 : 2) * kGroupWarps];
     __shared__ Prepared prepared[kPrepSlots];
     __shared__ int failed_word;
     volatile int* const failed = &failed_word;
@@ -410,9 +437,9 @@ distill_ring_kernel(const RingParams r) {
         }
         for (int i = 0; i < kPrepSlots; ++i) {
             mbar_init(&prep_full[i], 1);
-            mbar_init(&prep_empty[i], kConsumerWarps + 1);
+            mbar_init(&prep_empty[i], 2 * kGroupWarps + 1);
         }
-        for (int i = 0; i < 2; ++i) mbar_init(&stat_full[i], 1);
+        for (int i = 0; i < kStatSlots; ++i) mbar_init(&stat_full[i], 1);
         failed_word = 0;
         fence_mbar_init();
     }
@@ -453,7 +480,7 @@ distill_ring_kernel(const RingParams r) {
             }
         }
         __syncwarp();
-    } else if (warp < kFirstConsumer) {
+    } else if (warp < kFirstWorker) {
         // ---- the teacher's entries ----
         uint16_t* const table = tables + (warp - 1) * r.table;
         for (int64_t number = warp - 1; id + number * teams < p.rows; number += kPrepWarps) {
@@ -594,164 +621,74 @@ distill_ring_kernel(const RingParams r) {
             __syncwarp();
             if (lane == 0) mbar_arrive(&prep_full[place]);
         }
-    } else {
-        // ---- the logits ----
-        const int t = threadIdx.x - kFirstConsumer * kWarp, w = warp - kFirstConsumer;
-        const int group = w / kGroupWarps, tg = t % kGroup;
-        const float scale = p.scale * static_cast<float>(p.inv_temperature) *
-                            (GRAD && p.grad_loss != nullptr ? *p.grad_loss : 1.0f);
-        RingPlace slot{0, 0}, behind{0, 0};  // chunks of the current row, and of the row before (whose gradient lags)
-        RingPlace prep{0, 0}, prep_behind{0, 0};
-        uint32_t stat_round = 0;
-        struct Row {
-            int64_t row;
-            float m, total, coef;
-            float mass;
-        } cur{}, prev{};
-        bool has_prev = false, prev_phase = false;
-        T* pg = nullptr;
-        Slice<T> pslice(static_cast<const T*>(p.logits), p.vocab, rank, log2_cluster);
-
-        auto release = [&](int place) {  // this warp is done with the place
+    } else if (warp - kFirstWorker < kSumWarps) {
+        // ---- the sums ----
+        const int w = warp - kFirstWorker, group = w / kGroupWarps, tg = (w % kGroupWarps) * kWarp + lane;
+        RingPlace slot{0, 0}, prep{0, 0};
+        int64_t live_rows = 0;
+        struct Last {  // the loss alone: a row is closed after the sums of the next (warp 0)
+            int64_t row, number;
+            int place;
+        } last{-1, 0, 0};
+        auto row_of_stats = [&](int64_t number) { return &stat[number % kStatSlots][0]; };
+        auto close = [&]() {
+            if (!warp_wait<true>(&stat_full[last.number % kStatSlots], static_cast<uint32_t>(last.number / kStatSlots & 1), failed, r.error_flag)) return false;
+            const float2 f = fold_stats(row_of_stats(last.number), cluster * kSumWarps, c);
+            if (rank == 0 && lane == 0) write_loss(p, prepared[last.place], last.row, f);
             __syncwarp();
-            if (lane == 0) mbar_arrive(&empty[place]);
+            if (lane == 0) mbar_arrive(&prep_empty[last.place]);
+            last.row = -1;
+            return true;
         };
-        auto write_chunk = [&](const Row& row, const Slice<T>& slice, int i, int place, T* g, bool same_phase) {
-            const unsigned char* chunk = ring + static_cast<size_t>(place) * kChunkBytes;
-            const float each = row.coef * row.mass / row.total;
-            const int n = slice.size(i);
-            T* out = g + slice.head + static_cast<int64_t>(slice.begin(i)) * N;
-            if (same_phase) {
-                uint4 raw[kBatch];
-#pragma unroll
-                for (int q = 0; q < kBatch; ++q) raw[q] = reinterpret_cast<const uint4*>(chunk)[tg + q * kGroup];
-                const float2 down = both(-row.m), c2 = both(c), each2 = both(each);
-                T* const mine = out + static_cast<int64_t>(tg) * N;
-#pragma unroll
-                for (int q = 0; q < kBatch; ++q) {
-                    if (tg + q * kGroup >= n) break;
-                    float2 v[N / 2];
-                    unpack2(raw[q], v, T{});
-#pragma unroll
-                    for (int e = 0; e < N / 2; ++e) {
-                        v[e] = mul2(add2(v[e], down), c2);
-                        v[e] = mul2(make_float2(ex2_approx(v[e].x), ex2_approx(v[e].y)), each2);
-                    }
-                    store_pairs(mine + q * kGroup * N, v);
-                }
-            } else {
-                for (int q = tg; q < n * N; q += kGroup) {
-                    out[q] = from_f32<T>(ex2_approx((to_f32(reinterpret_cast<const T*>(chunk)[q]) - row.m) * c) * each);
-                }
-            }
-        };
-        auto write_edges = [&](const Row& row, const Slice<T>& slice, const Prepared& pre, T* g) {
-            if (rank == 0 && t < slice.edges()) {
-                g[slice.edge_col(t, p.vocab)] = from_f32<T>(ex2_approx((pre.edge[t] - row.m) * c) * (row.coef * row.mass / row.total));
-            }
-        };
-        // The columns that the teacher names: each warp writes those of its own share of the row again, so
-        // that no barrier has to come between them and the dense part.
-        auto write_named = [&](const Row& row, const Slice<T>& slice, int place, T* g, bool same_phase) {
-            __syncwarp();
-            for (int j = lane; j < p.k; j += kWarp) {
-                const int col = ats[place * p.k + j];
-                if (col < 0 || !slice.owns(col, rank)) continue;
-                int owner = 0;  // the edges: t < 16
-                if (slice.inner(col)) {
-                    const int pack = (col - slice.head) / N - slice.lo, in = pack % kChunkPacks;
-                    const int thread = (same_phase ? in : in * N + (col - slice.head) % N) % kGroup;
-                    owner = (pack / kChunkPacks % 2) * kGroupWarps + thread / kWarp;
-                }
-                if (owner != w) continue;
-                const float q = ex2_approx((heres[place * p.k + j] - row.m) * c) / row.total;
-                g[col] = from_f32<T>(row.coef * (row.mass * q - probs[place * p.k + j]));
-            }
-        };
-        auto phase_of = [&](const T* z, const T* g) {
-            return ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(g)) & 15) == 0;
-        };
-
-        for (int64_t at_row = id; at_row < p.rows || has_prev; at_row += teams) {
-            const bool has_cur = at_row < p.rows;
-            bool live = false;
-            if (has_cur) {
-                if (!warp_wait(&prep_full[prep.place], prep.parity, failed, r.error_flag)) break;
-                live = prepared[prep.place].live != 0;
-            }
-            const T* z = static_cast<const T*>(p.logits) + (has_cur ? at_row : id) * p.logits_stride;
-            const Slice<T> slice(z, p.vocab, rank, log2_cluster);
-            T* g = GRAD ? static_cast<T*>(p.grad) + (has_cur ? at_row : id) * p.grad_stride : nullptr;
-            cur.row = at_row;
+        for (int64_t row = id; row < p.rows; row += teams) {
+            if (!warp_wait(&prep_full[prep.place], prep.parity, failed, r.error_flag)) break;
+            const bool live = prepared[prep.place].live != 0;
+            bool keep = false;
             if (live) {
-                cur.coef = scale * prepared[prep.place].weight;
-                cur.mass = p.teacher_lse == nullptr ? 1.0f : static_cast<float>(prepared[prep.place].mass);
-                if (prepared[prep.place].mass != prepared[prep.place].mass) cur.mass = NAN;
-                if (!LOSS) {
-                    cur.m = prepared[prep.place].m;
-                    cur.total = prepared[prep.place].total;
-                }
-            }
-            float mx = -INFINITY, s = 0.0f;
-            auto take_chunk = [&](const uint4* chunk, int n) {
-                uint4 raw[kBatch];
+                const T* z = static_cast<const T*>(p.logits) + row * p.logits_stride;
+                const Slice<T> slice(z, p.vocab, rank, log2_cluster);
+                float mx = -INFINITY, s = 0.0f;
+                bool ok = true;
+                for (int i = 0; i < slice.chunks; ++i, slot.next(r.slots)) {
+                    if (kSumGroups > 1 && (i & 1) != group) continue;
+                    ok = warp_wait(&full[slot.place], slot.parity, failed, r.error_flag);
+                    if (!ok) break;
+                    const uint4* chunk = reinterpret_cast<const uint4*>(ring + static_cast<size_t>(slot.place) * kChunkBytes);
+                    const int n = slice.size(i);
+                    uint4 raw[kBatch];
 #pragma unroll
-                for (int q = 0; q < kBatch; ++q) raw[q] = tg + q * kGroup < n ? chunk[tg + q * kGroup] : lowest_pack(T{});
-                float big = -INFINITY;
-#pragma unroll
-                for (int q = 0; q < kBatch; ++q) {
-                    float2 v[N / 2];
-                    unpack2(raw[q], v, T{});
-#pragma unroll
-                    for (int e = 0; e < N / 2; ++e) big = fmaxf(big, fmaxf(v[e].x, v[e].y));
-                }
-                const float now = fmaxf(mx, big);
-                const float ref = now == -INFINITY ? 0.0f : now;  // nothing but -inf so far: exp(-inf) each
-                const float2 down = both(-ref), c2 = both(c);
-                float2 add[2] = {both(0.0f), both(0.0f)};
-#pragma unroll
-                for (int q = 0; q < kBatch; ++q) {
-                    float2 v[N / 2];
-                    unpack2(raw[q], v, T{});
-#pragma unroll
-                    for (int e = 0; e < N / 2; ++e) {
-                        v[e] = mul2(add2(v[e], down), c2);
-                        add[e & 1] = add2(add[e & 1], make_float2(ex2_approx(v[e].x), ex2_approx(v[e].y)));
+                    for (int q = 0; q < kBatch; ++q) raw[q] = tg + q * kGroup < n ? chunk[tg + q * kGroup] : lowest_pack(T{});
+                    if (!GRAD) {
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&empty[slot.place]);
                     }
-                }
-                const float2 sum = add2(add[0], add[1]);
-                s = s * exp_diff(mx, now, c) + (sum.x + sum.y);
-                mx = now;
-            };
-            const int steps = max(live ? slice.chunks : 0, kLag && has_prev ? pslice.chunks : 0);
-            const bool cur_phase = GRAD && phase_of(z, g);
-            bool ok = true;
-            for (int i = 0; i < steps; ++i) {
-                const bool mine = (i & 1) == group;  // the other group takes the other chunks
-                if (kLag && has_prev && i < pslice.chunks) {
-                    if (mine) {
-                        write_chunk(prev, pslice, i, behind.place, pg, prev_phase);
-                        release(behind.place);
+                    float big = -INFINITY;
+#pragma unroll
+                    for (int q = 0; q < kBatch; ++q) {
+                        float2 v[N / 2];
+                        unpack2(raw[q], v, T{});
+#pragma unroll
+                        for (int e = 0; e < N / 2; ++e) big = fmaxf(big, fmaxf(v[e].x, v[e].y));
                     }
-                    behind.next(r.slots);
-                }
-                if (live && i < slice.chunks) {
-                    if (mine) {
-                        ok = warp_wait(&full[slot.place], slot.parity, failed, r.error_flag);
-                        if (!ok) break;
-                        if (LOSS) {
-                            take_chunk(reinterpret_cast<const uint4*>(ring + static_cast<size_t>(slot.place) * kChunkBytes), slice.size(i));
-                            if (!GRAD) release(slot.place);
-                        } else {
-                            write_chunk(cur, slice, i, slot.place, g, cur_phase);
-                            release(slot.place);
+                    const float now = fmaxf(mx, big);
+                    const float ref = now == -INFINITY ? 0.0f : now;  // nothing but -inf so far: exp(-inf) each
+                    const float2 down = both(-ref), c2 = both(c);
+                    float2 add[2] = {both(0.0f), both(0.0f)};
+#pragma unroll
+                    for (int q = 0; q < kBatch; ++q) {
+                        float2 v[N / 2];
+                        unpack2(raw[q], v, T{});
+#pragma unroll
+                        for (int e = 0; e < N / 2; ++e) {
+                            v[e] = mul2(add2(v[e], down), c2);
+                            add[e & 1] = add2(add[e & 1], make_float2(ex2_approx(v[e].x), ex2_approx(v[e].y)));
                         }
                     }
-                    slot.next(r.slots);
+                    const float2 sum = add2(add[0], add[1]);
+                    s = s * exp_diff(mx, now, c) + (sum.x + sum.y);
+                    mx = now;
                 }
-            }
-            if (!ok) break;
-            if (live && LOSS) {
+                if (!ok) break;
                 if (rank == 0 && w == 0) {
                     const bool is_edge = lane < slice.edges();
                     const float v = is_edge ? prepared[prep.place].edge[lane] : -INFINITY;
@@ -761,75 +698,118 @@ distill_ring_kernel(const RingParams r) {
                 }
                 const float top = warp_max(mx);
                 const float2 mine = make_float2(top, warp_sum(s * exp_diff(mx, top, c)));
-                const int half = static_cast<int>(stat_round & 1u);
-                if (t == 0) mbar_expect_tx(&stat_full[half], static_cast<uint32_t>(cluster * kConsumerWarps * sizeof(float2)));
-                if (lane < cluster) send_stat(&stat[half][rank * kConsumerWarps + w], &stat_full[half], lane, mine);
-            }
-            if (kLag && has_prev) {  // while the sums travel
-                write_edges(prev, pslice, prepared[prep_behind.place], pg);
-                write_named(prev, pslice, prep_behind.place, pg, prev_phase);
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&prep_empty[prep_behind.place]);
-                prep_behind.next(kPrepSlots);
-            }
-            if (live && LOSS) {
-                const int half = static_cast<int>(stat_round & 1u);
-                if (!warp_wait<true>(&stat_full[half], (stat_round >> 1) & 1u, failed, r.error_flag)) break;
-                ++stat_round;
-                const int n = cluster * kConsumerWarps;
-                float m = -INFINITY;
-                for (int i = lane; i < n; i += kWarp) m = fmaxf(m, stat[half][i].x);
-                m = warp_max(m);
-                float sum = 0.0f;
-                for (int i = lane; i < n; i += kWarp) sum += stat[half][i].y * exp_diff(stat[half][i].x, m, c);
-                sum = warp_sum(sum);
-                cur.m = m;
-                cur.total = sum;
-                if (rank == 0 && t == 0) {
-                    p.row_stats[2 * at_row] = m;
-                    p.row_stats[2 * at_row + 1] = sum;
-                    const Prepared& pre = prepared[prep.place];
-                    p.row_loss[at_row] = static_cast<float>(
-                        pre.base + pre.mass * (static_cast<double>(m) * p.inv_temperature + log(static_cast<double>(sum))));
+                uint64_t* bar = &stat_full[live_rows % kStatSlots];
+                if (w == 0 && lane == 0) mbar_expect_tx(bar, static_cast<uint32_t>(cluster * kSumWarps * sizeof(float2)));
+                if (lane < cluster) send_stat(row_of_stats(live_rows) + rank * kSumWarps + w, bar, lane, mine);
+                if (!GRAD && w == 0) {
+                    if (last.row >= 0 && !close()) break;
+                    last = Last{row, live_rows, prep.place};
+                    keep = true;
                 }
+                ++live_rows;
+            } else if (!GRAD && rank == 0 && w == 0 && lane == 0) {
+                write_left_out(p, row);
             }
-            if (has_cur && !live) {  // left out
-                if (LOSS && rank == 0 && t == 0) {
-                    p.row_stats[2 * at_row] = 0.0f;
-                    p.row_stats[2 * at_row + 1] = 0.0f;
-                    p.row_loss[at_row] = 0.0f;
+            __syncwarp();
+            if (!keep && lane == 0) mbar_arrive(&prep_empty[prep.place]);
+            prep.next(kPrepSlots);
+        }
+        if (!GRAD && w == 0 && last.row >= 0 && *failed == 0) close();
+    } else {
+        // ---- the writes ----
+        const int w = warp - kFirstWorker - kSumWarps, group = w / kGroupWarps, tg = (w % kGroupWarps) * kWarp + lane;
+        const float scale = p.scale * static_cast<float>(p.inv_temperature) * (p.grad_loss != nullptr ? *p.grad_loss : 1.0f);
+        RingPlace slot{0, 0}, prep{0, 0};
+        int64_t live_rows = 0;
+        for (int64_t row = id; row < p.rows; row += teams) {
+            if (!warp_wait(&prep_full[prep.place], prep.parity, failed, r.error_flag)) break;
+            const Prepared& pre = prepared[prep.place];
+            const T* z = static_cast<const T*>(p.logits) + row * p.logits_stride;
+            T* g = static_cast<T*>(p.grad) + row * p.grad_stride;
+            const Slice<T> slice(z, p.vocab, rank, log2_cluster);
+            const bool same_phase = ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(g)) & 15) == 0;
+            T* const body = g + slice.head;
+            if (pre.live != 0) {
+                float2 f = make_float2(pre.m, pre.total);
+                if (LOSS) {
+                    if (!warp_wait<true>(&stat_full[live_rows % kStatSlots], static_cast<uint32_t>(live_rows / kStatSlots & 1), failed, r.error_flag)) break;
+                    f = fold_stats(&stat[live_rows % kStatSlots][0], cluster * kSumWarps, c);
+                    if (rank == 0 && w == 0 && lane == 0) write_loss(p, pre, row, f);
+                    ++live_rows;
                 }
-                if (GRAD) {
-                    T* out = g + slice.head + static_cast<int64_t>(slice.lo) * N;
-                    const int n = slice.hi - slice.lo;
-                    if (cur_phase) {
-                        for (int q = t; q < n; q += kConsumers) __stcs(reinterpret_cast<uint4*>(out) + q, make_uint4(0, 0, 0, 0));
+                const float m = f.x, total = f.y, coef = scale * pre.weight;
+                const float mass = p.teacher_lse == nullptr && pre.mass == pre.mass ? 1.0f : static_cast<float>(pre.mass);
+                const float each = coef * mass / total;
+                bool ok = true;
+                for (int i = 0; i < slice.chunks; ++i, slot.next(r.slots)) {
+                    if (kWriteGroups > 1 && (i & 1) != group) continue;
+                    ok = warp_wait(&full[slot.place], slot.parity, failed, r.error_flag);
+                    if (!ok) break;
+                    const unsigned char* chunk = ring + static_cast<size_t>(slot.place) * kChunkBytes;
+                    const int n = slice.size(i);
+                    T* const out = body + static_cast<int64_t>(slice.begin(i)) * N;
+                    if (same_phase) {
+                        uint4 raw[kBatch];
+#pragma unroll
+                        for (int q = 0; q < kBatch; ++q) raw[q] = reinterpret_cast<const uint4*>(chunk)[tg + q * kGroup];
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&empty[slot.place]);
+                        const float2 down = both(-m), c2 = both(c), each2 = both(each);
+                        T* const mine = out + static_cast<int64_t>(tg) * N;
+#pragma unroll
+                        for (int q = 0; q < kBatch; ++q) {
+                            if (tg + q * kGroup >= n) break;
+                            float2 v[N / 2];
+                            unpack2(raw[q], v, T{});
+#pragma unroll
+                            for (int e = 0; e < N / 2; ++e) {
+                                v[e] = mul2(add2(v[e], down), c2);
+                                v[e] = mul2(make_float2(ex2_approx(v[e].x), ex2_approx(v[e].y)), each2);
+                            }
+                            store_pairs(mine + q * kGroup * N, v);
+                        }
                     } else {
-                        for (int q = t; q < n * N; q += kConsumers) out[q] = from_f32<T>(0.0f);
+                        for (int q = tg; q < n * N; q += kGroup) {
+                            out[q] = from_f32<T>(ex2_approx((to_f32(reinterpret_cast<const T*>(chunk)[q]) - m) * c) * each);
+                        }
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&empty[slot.place]);
                     }
-                    if (rank == 0 && t < slice.edges()) g[slice.edge_col(t, p.vocab)] = from_f32<T>(0.0f);
                 }
-            }
-            if (!LOSS && live) {
-                write_edges(cur, slice, prepared[prep.place], g);
-                write_named(cur, slice, prep.place, g, cur_phase);
-            }
-            if (has_cur) {
-                has_prev = kLag && live;
-                if (has_prev) {
-                    prev = cur;
-                    prep_behind = prep;
-                    pslice = slice;
-                    pg = g;
-                    prev_phase = cur_phase;
+                if (!ok) break;
+                if (rank == 0 && w == 0 && lane < slice.edges()) {
+                    g[slice.edge_col(lane, p.vocab)] = from_f32<T>(ex2_approx((pre.edge[lane] - m) * c) * each);
+                }
+                // The columns that the teacher names: each warp writes those of its own share of the row again,
+                // so that no barrier has to come between them and the dense part.
+                __syncwarp();
+                for (int j = lane; j < p.k; j += kWarp) {
+                    const int col = ats[prep.place * p.k + j];
+                    if (col < 0 || !slice.owns(col, rank)) continue;
+                    int owner = 0;  // of the edges
+                    if (slice.inner(col)) {
+                        const int pack = (col - slice.head) / N - slice.lo, in = pack % kChunkPacks;
+                        owner = (same_phase ? in : in * N + (col - slice.head) % N) % kGroup / kWarp;
+                        if (kWriteGroups > 1) owner += pack / kChunkPacks % 2 * kGroupWarps;
+                    }
+                    if (owner != w) continue;
+                    const float q = ex2_approx((heres[prep.place * p.k + j] - m) * c) / total;
+                    g[col] = from_f32<T>(coef * (mass * q - probs[prep.place * p.k + j]));
+                }
+            } else {  // left out
+                if (LOSS && rank == 0 && w == 0 && lane == 0) write_left_out(p, row);
+                T* const out = body + static_cast<int64_t>(slice.lo) * N;
+                const int n = slice.hi - slice.lo, t = w * kWarp + lane;
+                if (same_phase) {
+                    for (int q = t; q < n; q += kWriteGroups * kGroup) __stcs(reinterpret_cast<uint4*>(out) + q, make_uint4(0, 0, 0, 0));
                 } else {
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&prep_empty[prep.place]);
+                    for (int q = t; q < n * N; q += kWriteGroups * kGroup) out[q] = from_f32<T>(0.0f);
                 }
-                prep.next(kPrepSlots);
-            } else {
-                has_prev = false;
+                if (rank == 0 && t < slice.edges()) g[slice.edge_col(t, p.vocab)] = from_f32<T>(0.0f);
             }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&prep_empty[prep.place]);
+            prep.next(kPrepSlots);
         }
     }
     __syncthreads();
