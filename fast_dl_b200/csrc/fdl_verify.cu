@@ -25,7 +25,7 @@ namespace fdl {
 
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / kWarp;
 constexpr int kMaxCluster = 8;
 
@@ -40,7 +40,6 @@ struct VerifyParams {
     const float* sample_u;
     int drafted;
     int vocab;
-    int run;  // elements of a warp's run
     int64_t* tokens;
     int64_t* accepted;
 };
@@ -67,57 +66,149 @@ __device__ __forceinline__ void store_remote(double* mine, uint32_t rank, double
     asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(remote), "d"(v) : "memory");
 }
 
-// What a row's weights are: p, max(p - q, 0), or p without one token.
+// What a row's weights are: p, max(p - q, 0), or p without one token.  Columns are taken in packs that lie on
+// the 16-byte grid of p's row: pack k holds the columns [k N - lead, (k + 1) N - lead), the first and the
+// last of them cut off by the row's ends.
 template <class T>
 struct Weights {
+    static constexpr int N = kPack<T>;
     const T* p;
-    const T* q;    // null: none
-    int without;   // -1: none
-    __device__ __forceinline__ double operator()(float pv, float qv, int col) const {
-        double w = static_cast<double>(pv);
-        if (q != nullptr) w -= static_cast<double>(qv);
-        if (col == without) w = 0.0;
-        return w > 0.0 && w < INFINITY ? w : 0.0;
+    const T* q;   // null: none
+    int without;  // -1: none
+    int vocab, lead;
+    bool q_packs;  // q's row lies on the same grid
+
+    __device__ __forceinline__ void set(const T* p_row, const T* q_row, int without_col, int n) {
+        p = p_row;
+        q = q_row;
+        without = without_col;
+        vocab = n;
+        lead = static_cast<int>((reinterpret_cast<uintptr_t>(p_row) & 15) / sizeof(T));
+        q_packs = ((reinterpret_cast<uintptr_t>(p_row) ^ reinterpret_cast<uintptr_t>(q_row)) & 15) == 0;
     }
-    __device__ __forceinline__ double at(int col) const {
-        return (*this)(to_f32(p[col]), q != nullptr ? to_f32(q[col]) : 0.0f, col);
-    }
-    // One lane's share of the sum over [lo, hi); `vec`: p, q and lo are on the 128-bit grid.
-    __device__ __forceinline__ double lane_sum(int lo, int hi, bool vec) const {
-        constexpr int N = kPack<T>;
-        const int lane = threadIdx.x & (kWarp - 1);
-        double s = 0.0;
-        int c = lo;
-        if (vec) {
-            const int packs = (hi - lo) / N;
-#pragma unroll 4
-            for (int i = lane; i < packs; i += kWarp) {
-                float a[N], b[N];
-                Chunk<T, N>::load(p + lo + i * N, a);
-                if (q != nullptr) {
-                    Chunk<T, N>::load(q + lo + i * N, b);
+    __device__ __forceinline__ int packs() const { return (vocab + lead + N - 1) / N; }
+
+    struct Loaded {
+        float a[N], b[N];
+    };
+    // The pack's values; 0 outside the row, and for k >= end.
+    __device__ __forceinline__ void load(int k, int end, Loaded& v) const {
+        const int col = k * N - lead;
+#pragma unroll
+        for (int e = 0; e < N; ++e) v.a[e] = v.b[e] = 0.0f;
+        if (k >= end) return;
+        if (col >= 0 && col + N <= vocab) {
+            Chunk<T, N>::load(p + col, v.a);
+            if (q != nullptr) {
+                if (q_packs) {
+                    Chunk<T, N>::load(q + col, v.b);
                 } else {
 #pragma unroll
-                    for (int e = 0; e < N; ++e) b[e] = 0.0f;
+                    for (int e = 0; e < N; ++e) v.b[e] = to_f32(q[col + e]);
                 }
-#pragma unroll
-                for (int e = 0; e < N; ++e) s += (*this)(a[e], b[e], lo + i * N + e);
             }
-            c = lo + packs * N;
+        } else {
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                if (col + e < 0 || col + e >= vocab) continue;
+                v.a[e] = to_f32(p[col + e]);
+                if (q != nullptr) v.b[e] = to_f32(q[col + e]);
+            }
         }
-#pragma unroll 8
-        for (int i = c + lane; i < hi; i += kWarp) s += at(i);
-        return s;
+    }
+    // The weight of element e of pack k: the exact difference where it is a positive number, 0 elsewhere.
+    __device__ __forceinline__ double weight(const Loaded& v, int k, int e) const {
+        const float d = v.a[e] - v.b[e];
+        const bool counts = d > 0.0f && d < INFINITY && k * N - lead + e != without;
+        return static_cast<double>(counts ? v.a[e] : 0.0f) - static_cast<double>(counts ? v.b[e] : 0.0f);
+    }
+    // One lane's share of the sum over the packs [lo, hi) of its warp.  As long as all weights are finite, each
+    // is max(p, q) - q (a NaN p drops out); one that is not makes the total infinite or NaN, and the caller asks
+    // again with kCareful, weight by weight.  That leaves five instructions a weight; with the tests in them
+    // it was 36, and the arithmetic, not the bytes, took the time.
+    template <bool kCareful>
+    __device__ __forceinline__ double lane_sum(int lo, int hi) const {
+        constexpr int kAhead = 4;  // packs of each row that a lane has on their way
+        const int lane = threadIdx.x & (kWarp - 1);
+        double s[4] = {0.0, 0.0, 0.0, 0.0};
+        const int whole_lo = lead > 0 ? 1 : 0, whole_hi = (vocab + lead) / N;  // packs that no end of the row cuts
+        if (kCareful) {
+#pragma unroll 1
+            for (int k = lo + lane; k < hi; k += kWarp) {
+                Loaded v;
+                load(k, hi, v);
+#pragma unroll
+                for (int e = 0; e < N; ++e) s[e & 3] += weight(v, k, e);
+            }
+            return (s[0] + s[1]) + (s[2] + s[3]);
+        }
+        const int from = max(lo, whole_lo), to = min(hi, whole_hi);
+#pragma unroll 1
+        for (int k0 = from + lane; k0 < to; k0 += kAhead * kWarp) {
+            uint4 a[kAhead], b[kAhead];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                a[u] = b[u] = make_uint4(0, 0, 0, 0);
+                const int k = k0 + u * kWarp;
+                if (k < to) {
+                    a[u] = *reinterpret_cast<const uint4*>(p + k * N - lead);
+                    if (q != nullptr) {
+                        if (q_packs) {
+                            b[u] = *reinterpret_cast<const uint4*>(q + k * N - lead);
+                        } else {
+                            T* const one = reinterpret_cast<T*>(&b[u]);
+#pragma unroll
+                            for (int e = 0; e < N; ++e) one[e] = q[k * N - lead + e];
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                float x[N], y[N];
+                unpack(a[u], x, T{});
+                if (q != nullptr) {
+                    unpack(b[u], y, T{});
+#pragma unroll
+                    for (int e = 0; e < N; ++e) s[e & 3] += static_cast<double>(fmaxf(x[e], y[e])) - static_cast<double>(y[e]);
+                } else {
+                    const unsigned int at = static_cast<unsigned int>(without - ((k0 + u * kWarp) * N - lead));
+#pragma unroll
+                    for (int e = 0; e < N; ++e) s[e & 3] += static_cast<double>(at == static_cast<unsigned int>(e) ? 0.0f : fmaxf(x[e], 0.0f));
+                }
+            }
+        }
+        // The packs that the row's ends cut.
+        const int cut = lane == 0 && lo < whole_lo ? 0 : lane == 1 && whole_hi < packs() && whole_hi >= from ? whole_hi : -1;
+        if (cut >= lo && cut < hi && (lane < 2)) {
+            Loaded v;
+            load(cut, hi, v);
+#pragma unroll
+            for (int e = 0; e < N; ++e) s[e & 3] += weight(v, cut, e);
+        }
+        return (s[0] + s[1]) + (s[2] + s[3]);
     }
 };
 
+__device__ __forceinline__ double warp_inclusive(double v) {
+    const int lane = threadIdx.x & (kWarp - 1);
+#pragma unroll
+    for (int o = 1; o < kWarp; o <<= 1) {
+        const double up = __shfl_up_sync(kFullMask, v, o);
+        if (lane >= o) v += up;
+    }
+    return v;
+}
+
 template <class T>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 4)
 verify_draft_kernel(const VerifyParams v) {
+    constexpr int N = kPack<T>;
+    constexpr int kRunsPerLane = kMaxCluster * kWarps / kWarp;  // 2
     __shared__ double run_sum[kMaxCluster * kWarps];  // of the whole row, in order
-    __shared__ double warp_total[kWarps];
+    __shared__ double warp_total[2][kWarps];
     __shared__ int first_rejected;
-    __shared__ int last_positive;
+    __shared__ int found, last_positive;
     const int t = threadIdx.x, lane = t & (kWarp - 1), warp = t / kWarp;
     const uint32_t rank = cluster_rank(), cluster = cluster_size();
     const int64_t b = blockIdx.x / cluster;
@@ -126,24 +217,25 @@ verify_draft_kernel(const VerifyParams v) {
     const T* target = static_cast<const T*>(v.target) + b * v.target_batch_stride;
     const T* draft = v.draft == nullptr ? nullptr : static_cast<const T*>(v.draft) + b * v.draft_batch_stride;
     const int64_t* drawn = v.draft_tokens + b * v.drafted;
-    int len = v.drafted;
-    if (v.draft_len != nullptr) {
-        const int64_t n = v.draft_len[b];
-        len = n < 0 ? 0 : n < v.drafted ? static_cast<int>(n) : v.drafted;
-    }
     // Every CTA of the cluster finds the first rejection by itself.
     if (warp == 0) {
+        int len = v.drafted;
+        if (v.draft_len != nullptr) {
+            const int64_t n = v.draft_len[b];
+            len = n < 0 ? 0 : n < v.drafted ? static_cast<int>(n) : v.drafted;
+        }
         int n = len;
         for (int base = 0; base < len; base += kWarp) {
             const int i = base + lane;
             bool ok = true;
             if (i < len) {
                 const int64_t d = drawn[i];
+                const float u = v.accept_u[b * v.drafted + i];
                 ok = d >= 0 && d < v.vocab;
                 if (ok) {
                     const float pd = to_f32(target[i * v.target_row_stride + d]);
                     const float qd = draft == nullptr ? 1.0f : to_f32(draft[i * v.draft_row_stride + d]);
-                    ok = __fmul_rn(v.accept_u[b * v.drafted + i], qd) < pd;
+                    ok = __fmul_rn(u, qd) < pd;
                 }
             }
             const unsigned int bad = __ballot_sync(kFullMask, !ok);
@@ -152,109 +244,136 @@ verify_draft_kernel(const VerifyParams v) {
                 break;
             }
         }
-        if (lane == 0) first_rejected = n;
+        if (lane == 0) {
+            first_rejected = n < len ? n : -1 - n;  // below 0: all stand
+            found = INT_MAX;
+            last_positive = -1;
+        }
     }
+    const float u_sample = v.sample_u[b];
     __syncthreads();
-    const int n = first_rejected;
+    const bool rejected = first_rejected >= 0;
+    const int n = rejected ? first_rejected : -1 - first_rejected;
     Weights<T> w;
-    w.p = target + n * v.target_row_stride;
-    w.q = n < len && draft != nullptr ? draft + n * v.draft_row_stride : nullptr;
-    w.without = -1;
-    if (n < len && draft == nullptr) {
-        const int64_t d = drawn[n];
-        w.without = d >= 0 && d < v.vocab ? static_cast<int>(d) : -1;
+    {
+        int without = -1;
+        if (rejected && draft == nullptr) {
+            const int64_t d = drawn[n];
+            without = d >= 0 && d < v.vocab ? static_cast<int>(d) : -1;
+        }
+        w.set(target + n * v.target_row_stride, rejected && draft != nullptr ? draft + n * v.draft_row_stride : nullptr, without,
+              v.vocab);
     }
     const int runs = static_cast<int>(cluster) * kWarps;
-    int64_t token = -1;
-    // The second round is for weights that are all 0 (the draft covers the target): the target's row itself.
-    for (int round = 0; round < 2; ++round) {
+    const int packs = w.packs();
+    const int run = (packs + runs - 1) / runs;
+    // Further rounds are for weights that are not all finite (careful), and for weights that are all 0 (the draft
+    // covers the target: the target's row itself).
+    bool careful = false, fallback = false;
+    for (int round = 0;; ++round) {
         const int mine = static_cast<int>(rank) * kWarps + warp;
-        const int64_t lo64 = static_cast<int64_t>(mine) * v.run;
-        const int lo = lo64 < v.vocab ? static_cast<int>(lo64) : v.vocab;
-        const int hi = v.vocab - lo < v.run ? v.vocab : lo + v.run;
-        const bool vec = ((reinterpret_cast<uintptr_t>(w.p) | reinterpret_cast<uintptr_t>(w.q)) & 15) == 0;
-        const double s = warp_sum(w.lane_sum(lo, hi, vec));
+        const int lo = min(packs, mine * run), hi_run = min(packs, (mine + 1) * run);
+        const double s = warp_sum(careful ? w.template lane_sum<true>(lo, hi_run) : w.template lane_sum<false>(lo, hi_run));
         if (round == 0) cluster_wait();
         if (lane < static_cast<int>(cluster)) store_remote(&run_sum[mine], lane, s);
         cluster_sync_all();
-        // Every thread walks the run sums in order: where the sum crosses, or else the last run with any weight.
-        double total = 0.0;
-        for (int r = 0; r < runs; ++r) total += run_sum[r];
-        if (total > 0.0) {
-            const double goal = static_cast<double>(v.sample_u[b]) * total;
-            double before = 0.0, base = 0.0, sum = 0.0;
-            int owner = -1;
-            bool crossed = false;
-            for (int r = 0; r < runs && !crossed; ++r) {
-                sum += run_sum[r];
-                if (run_sum[r] > 0.0) {
-                    owner = r;
-                    base = before;
-                    crossed = sum > goal;
-                }
-                before = sum;
-            }
-            if (owner / kWarps == static_cast<int>(rank)) {
-                // This CTA reads the run again, each thread a contiguous piece of it.
-                const int64_t start64 = static_cast<int64_t>(owner) * v.run;
-                const int start = static_cast<int>(start64);
-                const int stop = v.vocab - start < v.run ? v.vocab : start + v.run;
-                const int piece = (stop - start + kThreads - 1) / kThreads;
-                const int from = min(stop, start + t * piece), to = min(stop, from + piece);
-                double own = 0.0;
-                int last = -1;
-                for (int col = from; col < to; ++col) {
-                    const double x = w.at(col);
-                    own += x;
-                    if (x > 0.0) last = col;
-                }
-                double upto = own;  // inclusive over the warp
+        // Each warp walks the run sums, a few in a row to a lane: where the sum crosses the goal, or else the
+        // last run with any weight.
+        double part[kRunsPerLane];
+        double own = 0.0;
+        const int per_lane = (runs + kWarp - 1) / kWarp;
 #pragma unroll
-                for (int o = 1; o < kWarp; o <<= 1) {
-                    const double up = __shfl_up_sync(kFullMask, upto, o);
-                    if (lane >= o) upto += up;
-                }
-                if (lane == kWarp - 1) warp_total[warp] = upto;
-                if (t == 0) last_positive = -1;
-                __syncthreads();
-                for (int k = 0; k < warp; ++k) base += warp_total[k];
-                double reach = base + (upto - own);
-                int found = INT_MAX;
-                if (own > 0.0) {
-                    for (int col = from; col < to; ++col) {
-                        const double x = w.at(col);
-                        reach += x;
-                        if (x > 0.0 && reach > goal) {
-                            found = col;
-                            break;
-                        }
+        for (int i = 0; i < kRunsPerLane; ++i) {
+            part[i] = i < per_lane && lane * per_lane + i < runs ? run_sum[lane * per_lane + i] : 0.0;
+            own += part[i];
+        }
+        const double upto = warp_inclusive(own);
+        const double total = __shfl_sync(kFullMask, upto, kWarp - 1);
+        if (!careful && !(total < INFINITY)) {
+            careful = true;
+            cluster_sync_all();  // everybody has read the sums
+            continue;
+        }
+        if (total > 0.0) {
+            const double goal = static_cast<double>(u_sample) * total;
+            double sum = upto - own, base = 0.0;
+            int first = INT_MAX, last = -1;
+#pragma unroll
+            for (int i = 0; i < kRunsPerLane; ++i) {
+                if (part[i] > 0.0) {
+                    last = lane * per_lane + i;
+                    if (first == INT_MAX) {
+                        if (sum + part[i] > goal) first = last;
+                        else sum += part[i];
                     }
                 }
-                if (last >= 0) atomicMax(&last_positive, last);
-                found = __reduce_min_sync(kFullMask, found);
+            }
+            const int crossed = __reduce_min_sync(kFullMask, first);
+            const int owner = crossed != INT_MAX ? crossed : __reduce_max_sync(kFullMask, last);
+            base = __shfl_sync(kFullMask, sum, owner / per_lane);
+            if (crossed == INT_MAX) base = -INFINITY;  // the last weight, whatever the sum
+            if (owner / kWarps == static_cast<int>(rank)) {
+                // This CTA reads the run again in order, a pack a thread at a time.
+                const int hi = min(packs, (owner + 1) * run);
+                int half = 0;
+                for (int k0 = owner * run; k0 < hi; k0 += kThreads, half ^= 1) {
+                    const int k = k0 + t;
+                    typename Weights<T>::Loaded x;
+                    w.load(k, hi, x);
+                    double at[N];
+                    double mine_sum = 0.0;
+                    int last_col = -1;
+#pragma unroll
+                    for (int e = 0; e < N; ++e) {
+                        at[e] = w.weight(x, k, e);
+                        mine_sum += at[e];
+                        if (at[e] > 0.0) last_col = k * N - w.lead + e;
+                    }
+                    const double incl = warp_inclusive(mine_sum);
+                    if (lane == kWarp - 1) warp_total[half][warp] = incl;
+                    last_col = __reduce_max_sync(kFullMask, last_col);
+                    if (lane == 0 && last_col >= 0) atomicMax(&last_positive, last_col);
+                    __syncthreads();
+                    double before = 0.0, tile = 0.0;
+#pragma unroll
+                    for (int i = 0; i < kWarps; ++i) {
+                        if (i == warp) before = tile;
+                        tile += warp_total[half][i];
+                    }
+                    double reach = base + before + (incl - mine_sum);
+                    int hit = INT_MAX;
+#pragma unroll
+                    for (int e = N - 1; e >= 0; --e) {
+                        double to = reach;
+#pragma unroll
+                        for (int f = 0; f <= e; ++f) to += at[f];
+                        if (at[e] > 0.0 && to > goal) hit = k * N - w.lead + e;
+                    }
+                    hit = __reduce_min_sync(kFullMask, hit);
+                    if (lane == 0 && hit != INT_MAX) atomicMin(&found, hit);
+                    base += tile;
+                    if (__syncthreads_or(hit != INT_MAX)) break;
+                }
                 __syncthreads();
-                if (lane == 0) warp_total[warp] = static_cast<double>(found);
-                __syncthreads();
-                double best = warp_total[0];
-                for (int k = 1; k < kWarps; ++k) best = fmin(best, warp_total[k]);
-                // Rounding may leave the crossing to no one: the last weight of the run then.
-                token = best < static_cast<double>(INT_MAX) ? static_cast<int64_t>(best) : last_positive;
                 if (t == 0) {
-                    int64_t* out = v.tokens + b * (v.drafted + 1);
-                    out[n] = token;
+                    // Rounding may leave the crossing to no one: the last weight of the run then.
+                    v.tokens[b * (v.drafted + 1) + n] = found != INT_MAX ? found : last_positive;
                     v.accepted[b] = n;
                 }
             }
             break;
         }
-        if (round == 0) {
-            cluster_sync_all();  // everybody has read the sums
-            w.q = nullptr;
-            w.without = -1;
-        } else if (rank == 0 && t == 0) {
-            v.tokens[b * (v.drafted + 1) + n] = -1;
-            v.accepted[b] = n;
+        if (fallback) {
+            if (rank == 0 && t == 0) {
+                v.tokens[b * (v.drafted + 1) + n] = -1;
+                v.accepted[b] = n;
+            }
+            break;
         }
+        fallback = true;
+        careful = false;
+        cluster_sync_all();  // everybody has read the sums
+        w.set(w.p, nullptr, -1, v.vocab);
     }
     if (rank == 0) {
         int64_t* out = v.tokens + b * (v.drafted + 1);
@@ -292,12 +411,10 @@ int fdl_verify_draft(const void* target, int64_t target_batch_stride, int64_t ta
     if (info == nullptr) return status;
     // CTAs for each sequence: as many as leave a run of two packs a lane, while the batch does not fill the GPU.
     int cluster = 1;
-    while (cluster < kMaxCluster && batch * cluster * 2 <= 2 * info->sm_count && vocab > cluster * kThreads * 8) cluster *= 2;
-    const int64_t granule = 16 / static_cast<int64_t>(dtype_bytes(dtype));
-    const int64_t run = ceil_div(ceil_div(vocab, static_cast<int64_t>(cluster) * kWarps), granule) * granule;
+    while (cluster < kMaxCluster && batch * cluster * 2 <= 8 * info->sm_count && vocab > cluster * kThreads * 8) cluster *= 2;
     const VerifyParams p{target, target_batch_stride, target_row_stride, draft, draft_batch_stride, draft_row_stride,
                          draft_tokens, draft_len, accept_u, sample_u, static_cast<int>(drafted), static_cast<int>(vocab),
-                         static_cast<int>(run), tokens, accepted};
+                         tokens, accepted};
     return with_dtype(dtype, [&](auto* tag) {
         using T = std::remove_pointer_t<decltype(tag)>;
         return launch_ex(verify_draft_kernel<T>, dim3(static_cast<unsigned int>(batch * cluster)), dim3(kThreads), 0,
