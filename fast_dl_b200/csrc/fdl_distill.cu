@@ -299,7 +299,8 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
 // Stores (m, s) into CTA `rank`'s copy of `mine`, counted as eight bytes on its copy of `bar`.  (An ordinary
-// store and a releasing arrival would wait for the warp's gradient stores, a microsecond or two a row.)
+// store and a releasing arrival would wait for the warp's gradient stores, a microsecond or two a row.)  Only in a
+// launch with clusters: without one the instruction is not a legal one.
 __device__ __forceinline__ void send_stat(float2* mine, uint64_t* bar, uint32_t rank, float2 v) {
     uint32_t to, at;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_addr(mine)), "r"(rank));
@@ -337,6 +338,11 @@ __device__ __forceinline__ bool lane_wait(uint64_t* bar, uint32_t parity, volati
 template <bool CLUSTER = false>
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* failed, unsigned int* error_flag) {
     return __all_sync(kFullMask, lane_wait<CLUSTER>(bar, parity, failed, error_flag));
+}
+
+// For the pairs of a row: from all CTAs of the cluster.
+__device__ __forceinline__ bool stat_wait(int cluster, uint64_t* bar, uint32_t parity, volatile int* failed, unsigned int* error_flag) {
+    return cluster == 1 ? warp_wait(bar, parity, failed, error_flag) : warp_wait<true>(bar, parity, failed, error_flag);
 }
 
 // -inf in each element of a pack.
@@ -439,7 +445,7 @@ distill_ring_kernel(const RingParams r) {
             mbar_init(&prep_full[i], 1);
             mbar_init(&prep_empty[i], 2 * kGroupWarps + 1);
         }
-        for (int i = 0; i < kStatSlots; ++i) mbar_init(&stat_full[i], 1);
+        for (int i = 0; i < kStatSlots; ++i) mbar_init(&stat_full[i], cluster == 1 && LOSS ? kSumWarps : 1);
         failed_word = 0;
         fence_mbar_init();
     }
@@ -632,7 +638,7 @@ distill_ring_kernel(const RingParams r) {
         } last{-1, 0, 0};
         auto row_of_stats = [&](int64_t number) { return &stat[number % kStatSlots][0]; };
         auto close = [&]() {
-            if (!warp_wait<true>(&stat_full[last.number % kStatSlots], static_cast<uint32_t>(last.number / kStatSlots & 1), failed, r.error_flag)) return false;
+            if (!stat_wait(cluster, &stat_full[last.number % kStatSlots], static_cast<uint32_t>(last.number / kStatSlots & 1), failed, r.error_flag)) return false;
             const float2 f = fold_stats(row_of_stats(last.number), cluster * kSumWarps, c);
             if (rank == 0 && lane == 0) write_loss(p, prepared[last.place], last.row, f);
             __syncwarp();
@@ -699,8 +705,15 @@ distill_ring_kernel(const RingParams r) {
                 const float top = warp_max(mx);
                 const float2 mine = make_float2(top, warp_sum(s * exp_diff(mx, top, c)));
                 uint64_t* bar = &stat_full[live_rows % kStatSlots];
-                if (w == 0 && lane == 0) mbar_expect_tx(bar, static_cast<uint32_t>(cluster * kSumWarps * sizeof(float2)));
-                if (lane < cluster) send_stat(row_of_stats(live_rows) + rank * kSumWarps + w, bar, lane, mine);
+                if (cluster == 1) {  // launched without a cluster: nothing but the CTA's own shared memory
+                    if (lane == 0) {
+                        row_of_stats(live_rows)[w] = mine;
+                        mbar_arrive(bar);
+                    }
+                } else {
+                    if (w == 0 && lane == 0) mbar_expect_tx(bar, static_cast<uint32_t>(cluster * kSumWarps * sizeof(float2)));
+                    if (lane < cluster) send_stat(row_of_stats(live_rows) + rank * kSumWarps + w, bar, lane, mine);
+                }
                 if (!GRAD && w == 0) {
                     if (last.row >= 0 && !close()) break;
                     last = Last{row, live_rows, prep.place};
@@ -732,7 +745,7 @@ distill_ring_kernel(const RingParams r) {
             if (pre.live != 0) {
                 float2 f = make_float2(pre.m, pre.total);
                 if (LOSS) {
-                    if (!warp_wait<true>(&stat_full[live_rows % kStatSlots], static_cast<uint32_t>(live_rows / kStatSlots & 1), failed, r.error_flag)) break;
+                    if (!stat_wait(cluster, &stat_full[live_rows % kStatSlots], static_cast<uint32_t>(live_rows / kStatSlots & 1), failed, r.error_flag)) break;
                     f = fold_stats(&stat[live_rows % kStatSlots][0], cluster * kSumWarps, c);
                     if (rank == 0 && w == 0 && lane == 0) write_loss(p, pre, row, f);
                     ++live_rows;
