@@ -664,10 +664,6 @@ distill_ring_kernel(const RingParams r) {
                     uint4 raw[kBatch];
 #pragma unroll
                     for (int q = 0; q < kBatch; ++q) raw[q] = tg + q * kGroup < n ? chunk[tg + q * kGroup] : lowest_pack(T{});
-                    if (!GRAD) {
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&empty[slot.place]);
-                    }
                     float big = -INFINITY;
 #pragma unroll
                     for (int q = 0; q < kBatch; ++q) {
@@ -693,6 +689,9 @@ distill_ring_kernel(const RingParams r) {
                     const float2 sum = add2(add[0], add[1]);
                     s = s * exp_diff(mx, now, c) + (sum.x + sum.y);
                     mx = now;
+                    // The place is given back once every lane's loads have returned, not when they are under way: the
+                    // vote needs sums of all of them (a sum is never -1).
+                    if (!GRAD && !__any_sync(kFullMask, s == -1.0f) && lane == 0) mbar_arrive(&empty[slot.place]);
                 }
                 if (!ok) break;
                 if (rank == 0 && w == 0) {
@@ -720,8 +719,10 @@ distill_ring_kernel(const RingParams r) {
                     keep = true;
                 }
                 ++live_rows;
-            } else if (!GRAD && rank == 0 && w == 0 && lane == 0) {
-                write_left_out(p, row);
+            } else if (!GRAD && w == 0) {
+                // Slots are given back in the order of their rows: their barriers tell one round from the next only.
+                if (last.row >= 0 && !close()) break;
+                if (rank == 0 && lane == 0) write_left_out(p, row);
             }
             __syncwarp();
             if (!keep && lane == 0) mbar_arrive(&prep_empty[prep.place]);
@@ -765,8 +766,6 @@ distill_ring_kernel(const RingParams r) {
                         uint4 raw[kBatch];
 #pragma unroll
                         for (int q = 0; q < kBatch; ++q) raw[q] = reinterpret_cast<const uint4*>(chunk)[tg + q * kGroup];
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&empty[slot.place]);
                         const float2 down = both(-m), c2 = both(c), each2 = both(each);
                         T* const mine = out + static_cast<int64_t>(tg) * N;
 #pragma unroll
@@ -785,9 +784,11 @@ distill_ring_kernel(const RingParams r) {
                         for (int q = tg; q < n * N; q += kGroup) {
                             out[q] = from_f32<T>(ex2_approx((to_f32(reinterpret_cast<const T*>(chunk)[q]) - m) * c) * each);
                         }
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&empty[slot.place]);
                     }
+                    // Behind the stores, which need what the lanes loaded: a place given back while loads are still
+                    // under way is overwritten under them.
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&empty[slot.place]);
                 }
                 if (!ok) break;
                 if (rank == 0 && w == 0 && lane < slice.edges()) {

@@ -750,7 +750,7 @@ norm_residual_ring_kernel(const NormParams p, const RingPlan plan) {
         }
         const float2 s2 = moments(p.pre_kind);
         if (p.pre_kind == FDL_NORM_NONE) __syncthreads();
-        // Behind a barrier that follows everybody's reads of the stage.
+        // Behind a barrier that follows the use of everything that was loaded from the stage.
         if (t == 0 && row + plan.stages < to && !ring.failed) request(row + plan.stages, ring.stage);
         if (p.stats != nullptr && t == 0 && team.rank == 0) {
             reinterpret_cast<float4*>(p.stats)[row] = make_float4(s1.x, s1.y, s2.x, s2.y);
@@ -996,9 +996,8 @@ norm_residual_backward_ring_kernel(const NormParams p, const RingPlan plan) {
                 }
             }
             float s[2] = {sd.x + sd.y, sh.x + sh.y};
-            if (p.post_kind != FDL_NORM_NONE) team.sum(s);
-            else __syncthreads();
-            if (t == 0 && !ring.failed) request(ring.stage);  // everybody has read the stage
+            team.sum(s);  // (also where no norm needs it: the sums need all that was loaded)
+            if (t == 0 && !ring.failed) request(ring.stage);  // everybody's loads of the stage have returned
             if (p.dh != nullptr) {
                 level = p.post_kind == FDL_NORM_LAYER ? s[0] * inv : 0.0f;
                 along = p.post_kind != FDL_NORM_NONE ? s[1] * inv : 0.0f;

@@ -144,6 +144,29 @@ def test_padding_entries_rows_and_weights(fdl, cuda, kind):
             assert not stats[r].any()
 
 
+@pytest.mark.parametrize("kind,rows,vocab", [("f32", 1300, 4200), ("bf16", 1100, 8200), ("f16", 2500, 300), ("f32", 600, 20000)])
+def test_many_rows_with_some_left_out(fdl, cuda, kind, rows, vocab):
+    """Many rows a CTA, single rows and runs of rows left out, in each of the three calls."""
+    k = 6
+    z, t, index, _ = make(rows, vocab, k, kind, seed=rows)
+    g = torch.Generator().manual_seed(5)
+    weight = torch.ones(rows)
+    weight[torch.rand(rows, generator=g) < 0.3] = 0.0
+    weight[rows // 2:] = (torch.rand(rows - rows // 2, generator=g) < 0.2).float()
+    weight = weight.cuda()
+    index[::7] = -1
+    z[::7] = float("nan")
+    want_rows, want, want_grad, info = definition(z, t, index, None, weight, 1.0, 0.5)
+    for _ in range(3):
+        loss, row_loss, stats = fdl.distill_topk(z, t, index, row_weight=weight, scale=0.5)
+        check_loss(row_loss, loss, want_rows, want, info, vocab, weight, 0.5)
+        check_grad(fdl.distill_topk_backward(z, t, index, stats, row_weight=weight, scale=0.5), want_grad, info, vocab, kind)
+        loss, row_loss, grad = fdl.distill_topk_with_grad(z, t, index, row_weight=weight, scale=0.5)
+        check_loss(row_loss, loss, want_rows, want, info, vocab, weight, 0.5)
+        check_grad(grad, want_grad, info, vocab, kind)
+    fdl.take_device_error()
+
+
 def test_no_row_at_all_counts_and_no_rows(fdl, cuda):
     z, t, index, _ = make(3, 100, 4, "f32")
     loss, row_loss, grad = fdl.distill_topk_with_grad(z, t, torch.full_like(index, -1))
