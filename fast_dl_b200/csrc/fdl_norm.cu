@@ -531,8 +531,10 @@ constexpr int kMaxStages = 4;
 
 struct RingPlan {
     int stages;
-    int tiles;        // tensors a stage holds
-    int slice_packs;  // packs of a row that a CTA of the cluster owns
+    int tiles;    // tensors a stage holds
+    int slice;    // what a CTA of the cluster owns of a row: 128-bit packs, or columns (rows off the 16-byte grid)
+    int tile;     // 128-bit words of a tensor's place in a stage
+    int weights;  // floats of a weight's place
 };
 
 template <int NV>
@@ -597,51 +599,141 @@ struct RingWait {
     }
 };
 
-// The floats of pack i, kept as N / 4 arrays of 128-bit groups so that lanes next to each other read next
-// to each other.
-template <int M>
-__device__ __forceinline__ void load_floats(const float4* w, int i, int packs, float2 (&v)[M]) {
-#pragma unroll
-    for (int q = 0; q < M / 2; ++q) {
-        const float4 f = w[q * packs + i];
-        v[2 * q] = make_float2(f.x, f.y);
-        v[2 * q + 1] = make_float2(f.z, f.w);
-    }
-}
-template <int M>
-__device__ __forceinline__ void keep_floats(float4* w, int i, int packs, const float2 (&v)[M]) {
-#pragma unroll
-    for (int q = 0; q < M / 2; ++q) w[q * packs + i] = make_float4(v[2 * q].x, v[2 * q].y, v[2 * q + 1].x, v[2 * q + 1].y);
-}
-// w[col ...] (on the 16-byte grid), or ones where there is no w.
-template <int M>
-__device__ __forceinline__ void fetch_floats(const float* w, int col, float2 (&v)[M]) {
-#pragma unroll
-    for (int q = 0; q < M / 2; ++q) {
-        const float4 f = w != nullptr ? __ldg(reinterpret_cast<const float4*>(w + col) + q) : make_float4(1.0f, 1.0f, 1.0f, 1.0f);
-        v[2 * q] = make_float2(f.x, f.y);
-        v[2 * q + 1] = make_float2(f.z, f.w);
-    }
-}
+// The columns of a thread, N at a time.  VEC: rows are whole packs on the 16-byte grid, and N is a pack's columns.
+// Otherwise 8 columns a team's width apart, element by element: every row then starts at another place of
+// a 16-byte word, and a tile holds the words that cover it.
+template <class T, bool VEC>
+struct Columns {
+    static constexpr int N = VEC ? kPack<T> : 8, M = N / 2;
+    int t, threads;
+    int first, count;  // packs (VEC) or columns
 
-template <class T, int PACKS>
+    __device__ __forceinline__ int at(int k) const { return t + k * threads; }
+    __device__ __forceinline__ bool has(int k) const { return at(k) < count; }
+    __device__ __forceinline__ bool inside(int e) const { return VEC || t + e * threads < count; }
+    __device__ __forceinline__ int col(int k, int e) const { return VEC ? (first + at(k)) * N + e : first + t + e * threads; }
+
+    // Where a row of this slice begins in memory, and how many bytes its tile takes, from `total` bytes of tensor.
+    struct Span {
+        size_t from;
+        uint32_t bytes;
+        int lead;  // elements before the slice's first in the tile
+        int safe;  // columns that the tile has (all but the last few of the tensor's last row)
+    };
+    __device__ __forceinline__ Span span(int64_t row, int cols, int64_t rows) const {
+        if (VEC) {
+            return {(static_cast<size_t>(row) * cols + static_cast<size_t>(first) * N) * sizeof(T), static_cast<uint32_t>(count) * 16u, 0,
+                    count};
+        }
+        const size_t begin = (static_cast<size_t>(row) * cols + first) * sizeof(T);
+        const size_t from = begin & ~static_cast<size_t>(15);
+        size_t end = (begin + static_cast<size_t>(count) * sizeof(T) + 15) & ~static_cast<size_t>(15);
+        const size_t total = static_cast<size_t>(rows) * cols * sizeof(T) & ~static_cast<size_t>(15);
+        if (end > total) end = total;
+        return {from, static_cast<uint32_t>(end - from), static_cast<int>((begin - from) / sizeof(T)),
+                static_cast<int>((end - begin) / sizeof(T))};
+    }
+    __device__ __forceinline__ void load(const uint4* tile, const Span& s, const T* row, int k, float2 (&v)[M]) const {
+        if constexpr (VEC) {
+            unpack2(has(k) ? tile[at(k)] : make_uint4(0, 0, 0, 0), v, T{});
+        } else {
+            float f[N];
+            const T* from = reinterpret_cast<const T*>(tile) + s.lead + t;
+#pragma unroll
+            for (int e = 0; e < N; ++e) f[e] = inside(e) && t + e * threads < s.safe ? to_f32(from[e * threads]) : 0.0f;
+            if (s.safe < count) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    if (inside(e) && t + e * threads >= s.safe) f[e] = to_f32(row[col(k, e)]);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < M; ++e) v[e] = make_float2(f[2 * e], f[2 * e + 1]);
+        }
+    }
+    __device__ __forceinline__ void load_row(const T* row, int k, float2 (&v)[M]) const {
+        if constexpr (VEC) {
+            unpack2(__ldg(reinterpret_cast<const uint4*>(row + col(k, 0))), v, T{});
+        } else {
+            float f[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) f[e] = inside(e) ? to_f32(row[col(k, e)]) : 0.0f;
+#pragma unroll
+            for (int e = 0; e < M; ++e) v[e] = make_float2(f[2 * e], f[2 * e + 1]);
+        }
+    }
+    __device__ __forceinline__ void store(T* row, int k, const float2 (&v)[M]) const {
+        if constexpr (VEC) {
+            store_pairs(row + col(k, 0), v);
+        } else {
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                if (inside(e)) __stcs(row + col(k, e), from_f32<T>(e % 2 == 0 ? v[e / 2].x : v[e / 2].y));
+            }
+        }
+    }
+    // A weight's floats of these columns (ones where there is no weight, 0 outside the row).
+    __device__ __forceinline__ void fetch(const float* w, int k, float2 (&v)[M]) const {
+        if constexpr (VEC) {
+#pragma unroll
+            for (int q = 0; q < M / 2; ++q) {
+                const float4 f = w != nullptr ? __ldg(reinterpret_cast<const float4*>(w + col(k, 0)) + q) : make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+                v[2 * q] = make_float2(f.x, f.y);
+                v[2 * q + 1] = make_float2(f.z, f.w);
+            }
+        } else {
+            float f[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) f[e] = !inside(e) ? 0.0f : w != nullptr ? __ldg(w + col(k, e)) : 1.0f;
+#pragma unroll
+            for (int e = 0; e < M; ++e) v[e] = make_float2(f[2 * e], f[2 * e + 1]);
+        }
+    }
+    // The same floats in shared memory: N / 4 arrays of 128-bit groups (VEC: lanes next to each other read next to
+    // each other), or one column after the other.
+    __device__ __forceinline__ void keep(float* w, int k, const float2 (&v)[M]) const {
+        if constexpr (VEC) {
+#pragma unroll
+            for (int q = 0; q < M / 2; ++q) {
+                reinterpret_cast<float4*>(w)[q * count + at(k)] = make_float4(v[2 * q].x, v[2 * q].y, v[2 * q + 1].x, v[2 * q + 1].y);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < N; ++e) w[t + e * threads] = e % 2 == 0 ? v[e / 2].x : v[e / 2].y;
+        }
+    }
+    __device__ __forceinline__ void kept(const float* w, int k, float2 (&v)[M]) const {
+        if constexpr (VEC) {
+#pragma unroll
+            for (int q = 0; q < M / 2; ++q) {
+                const float4 f = reinterpret_cast<const float4*>(w)[q * count + at(k)];
+                v[2 * q] = make_float2(f.x, f.y);
+                v[2 * q + 1] = make_float2(f.z, f.w);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < M; ++e) v[e] = make_float2(w[t + 2 * e * threads], w[t + (2 * e + 1) * threads]);
+        }
+    }
+};
+
+template <class T, int PACKS, bool VEC>
 __global__ void __launch_bounds__(512, 2)
 norm_residual_ring_kernel(const NormParams p, const RingPlan plan) {
-    constexpr int N = kPack<T>, M = N / 2;
+    constexpr int M = Columns<T, VEC>::M;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ RingSums<1> sums;
     __shared__ uint64_t full[kMaxStages];
     RingTeam<1> team{&sums, 0, static_cast<int>(blockDim.x) / kWarp, static_cast<int>(cluster_size()),
                      static_cast<int>(cluster_rank())};
-    const int t = threadIdx.x, threads = blockDim.x;
-    const int row_packs = p.cols / N, slice = plan.slice_packs;
-    const int first = team.rank * slice;
-    const int count = min(slice, row_packs - first);
+    const int t = threadIdx.x;
+    const int units = VEC ? p.cols / kPack<T> : p.cols;
+    const Columns<T, VEC> own{t, static_cast<int>(blockDim.x), team.rank * plan.slice, min(plan.slice, units - team.rank * plan.slice)};
     const int64_t teams = gridDim.x / team.cluster, id = blockIdx.x / team.cluster;
     const int64_t from = p.rows * id / teams, to = p.rows * (id + 1) / teams;
     const bool gate_each = p.gate != nullptr && p.rows_per_gate == 1;
     const bool gate_shared = p.gate != nullptr && !gate_each;
-    uint4* const stages = reinterpret_cast<uint4*>(smem);  // [stages][tiles][slice]
+    uint4* const stages = reinterpret_cast<uint4*>(smem);  // [stages][tiles][tile]
     if (t == 0) {
         for (int s = 0; s < plan.stages; ++s) mbar_init(&full[s], 1);
         fence_mbar_init();
@@ -650,12 +742,12 @@ norm_residual_ring_kernel(const NormParams p, const RingPlan plan) {
     else __syncthreads();
     pdl_wait();
     auto request = [&](int64_t row, int stage) {
-        const size_t at = (static_cast<size_t>(row) * p.cols + static_cast<size_t>(first) * N) * sizeof(T);
-        uint4* tile = stages + static_cast<size_t>(stage) * plan.tiles * slice;
-        mbar_expect_tx(&full[stage], static_cast<uint32_t>(plan.tiles * count * 16));
-        bulk_g2s(tile, static_cast<const unsigned char*>(p.h) + at, count * 16, &full[stage]);
-        bulk_g2s(tile + slice, static_cast<const unsigned char*>(p.x) + at, count * 16, &full[stage]);
-        if (gate_each) bulk_g2s(tile + 2 * slice, static_cast<const unsigned char*>(p.gate) + at, count * 16, &full[stage]);
+        const auto span = own.span(row, p.cols, p.rows);
+        uint4* tile = stages + static_cast<size_t>(stage) * plan.tiles * plan.tile;
+        mbar_expect_tx(&full[stage], static_cast<uint32_t>(plan.tiles) * span.bytes);
+        bulk_g2s(tile, static_cast<const unsigned char*>(p.h) + span.from, span.bytes, &full[stage]);
+        bulk_g2s(tile + plan.tile, static_cast<const unsigned char*>(p.x) + span.from, span.bytes, &full[stage]);
+        if (gate_each) bulk_g2s(tile + 2 * plan.tile, static_cast<const unsigned char*>(p.gate) + span.from, span.bytes, &full[stage]);
     };
     if (t == 0) {
         for (int s = 0; s < plan.stages && from + s < to; ++s) request(from + s, s);
@@ -663,26 +755,21 @@ norm_residual_ring_kernel(const NormParams p, const RingPlan plan) {
     RingWait ring{full, plan.stages, 0, 0, false};
     const float inv = 1.0f / static_cast<float>(p.cols);
     const float2 residual = both(p.residual_scale);
-    // This thread's first column in the current row, and of the shared gate's row.
-    const int64_t start = from * p.cols + static_cast<int64_t>(first + t) * N;
-    T* y = static_cast<T*>(p.y) + start;
-    T* n = p.n != nullptr ? static_cast<T*>(p.n) + start : nullptr;
-    const T* gate = nullptr;
-    int64_t gate_left = 0;  // rows that the gate's row still serves
+    const T* gate = nullptr;  // the row of a shared gate
+    int64_t gate_left = 0;    // rows that it still serves
     if (gate_shared && from < to) {
         const int64_t group = from / p.rows_per_gate;
-        gate = static_cast<const T*>(p.gate) + group * p.cols + static_cast<int64_t>(first + t) * N;
+        gate = static_cast<const T*>(p.gate) + group * p.cols;
         gate_left = (group + 1) * p.rows_per_gate - from;
     }
-    for (int64_t row = from; row < to; ++row, y += p.cols, n += p.n != nullptr ? p.cols : 0) {
+    for (int64_t row = from; row < to; ++row) {
+        const int64_t base = row * p.cols;
+        const auto span = own.span(row, p.cols, p.rows);
         ring.wait(p.error_flag);
-        const uint4* tile = stages + ring.stage * plan.tiles * slice;
+        const uint4* tile = stages + ring.stage * plan.tiles * plan.tile;
         float2 v[PACKS][M];
 #pragma unroll
-        for (int k = 0; k < PACKS; ++k) {
-            const int i = t + k * threads;
-            unpack2(i < count ? tile[i] : make_uint4(0, 0, 0, 0), v[k], T{});
-        }
+        for (int k = 0; k < PACKS; ++k) own.load(tile, span, static_cast<const T*>(p.h) + base, k, v[k]);
         auto moments = [&](int kind) {
             if (kind == FDL_NORM_NONE) return make_float2(0.0f, 1.0f);
             float mean = 0.0f;
@@ -699,10 +786,12 @@ norm_residual_ring_kernel(const NormParams p, const RingPlan plan) {
                 mean = s[0] * inv;
 #pragma unroll
                 for (int k = 0; k < PACKS; ++k) {
-                    if (t + k * threads >= count) continue;
+                    if (!own.has(k)) continue;
 #pragma unroll
                     for (int e = 0; e < M; ++e) {
-                        const float2 c = add2(v[k][e], both(-mean));
+                        float2 c = add2(v[k][e], both(-mean));
+                        if (!own.inside(2 * e)) c.x = 0.0f;
+                        if (!own.inside(2 * e + 1)) c.y = 0.0f;
                         q2 = fma2(c, c, q2);
                     }
                 }
@@ -722,31 +811,35 @@ norm_residual_ring_kernel(const NormParams p, const RingPlan plan) {
         const float2 r1 = both(s1.y * p.block_scale), shift1 = both(-s1.x * s1.y * p.block_scale);
 #pragma unroll
         for (int k = 0; k < PACKS; ++k) {
-            const int i = t + k * threads;
-            if (i >= count) continue;
+            if (!own.has(k)) continue;
             float2 w[M];
 #pragma unroll
             for (int e = 0; e < M; ++e) v[k][e] = fma2(v[k][e], r1, shift1);
             if (p.post_gamma != nullptr) {
-                fetch_floats(p.post_gamma, (first + i) * N, w);
+                own.fetch(p.post_gamma, k, w);
 #pragma unroll
                 for (int e = 0; e < M; ++e) v[k][e] = mul2(v[k][e], w[e]);
             }
             if (p.post_beta != nullptr) {
-                fetch_floats(p.post_beta, (first + i) * N, w);
+                own.fetch(p.post_beta, k, w);
 #pragma unroll
                 for (int e = 0; e < M; ++e) v[k][e] = fma2(both(p.block_scale), w[e], v[k][e]);
             }
             if (p.gate != nullptr) {
-                unpack2(gate_each ? tile[2 * slice + i] : __ldg(reinterpret_cast<const uint4*>(gate) + k * threads), w, T{});
+                if (gate_each) own.load(tile + 2 * plan.tile, span, static_cast<const T*>(p.gate) + base, k, w);
+                else own.load_row(gate, k, w);
                 gate_pairs(p.gate_act, w);
 #pragma unroll
                 for (int e = 0; e < M; ++e) v[k][e] = mul2(v[k][e], w[e]);
             }
-            unpack2(tile[slice + i], w, T{});
+            own.load(tile + plan.tile, span, static_cast<const T*>(p.x) + base, k, w);
 #pragma unroll
-            for (int e = 0; e < M; ++e) v[k][e] = fma2(residual, w[e], v[k][e]);
-            store_pairs(y + k * threads * N, v[k]);
+            for (int e = 0; e < M; ++e) {
+                v[k][e] = fma2(residual, w[e], v[k][e]);
+                if (!own.inside(2 * e)) v[k][e].x = 0.0f;
+                if (!own.inside(2 * e + 1)) v[k][e].y = 0.0f;
+            }
+            own.store(static_cast<T*>(p.y) + base, k, v[k]);
         }
         const float2 s2 = moments(p.pre_kind);
         if (p.pre_kind == FDL_NORM_NONE) __syncthreads();
@@ -759,22 +852,21 @@ norm_residual_ring_kernel(const NormParams p, const RingPlan plan) {
             const float2 r2 = both(s2.y), shift2 = both(-s2.x * s2.y);
 #pragma unroll
             for (int k = 0; k < PACKS; ++k) {
-                const int i = t + k * threads;
-                if (i >= count) continue;
+                if (!own.has(k)) continue;
                 float2 w[M];
 #pragma unroll
                 for (int e = 0; e < M; ++e) v[k][e] = fma2(v[k][e], r2, shift2);
                 if (p.pre_gamma != nullptr) {
-                    fetch_floats(p.pre_gamma, (first + i) * N, w);
+                    own.fetch(p.pre_gamma, k, w);
 #pragma unroll
                     for (int e = 0; e < M; ++e) v[k][e] = mul2(v[k][e], w[e]);
                 }
                 if (p.pre_beta != nullptr) {
-                    fetch_floats(p.pre_beta, (first + i) * N, w);
+                    own.fetch(p.pre_beta, k, w);
 #pragma unroll
                     for (int e = 0; e < M; ++e) v[k][e] = add2(v[k][e], w[e]);
                 }
-                store_pairs(n + k * threads * N, v[k]);
+                own.store(static_cast<T*>(p.n) + base, k, v[k]);
             }
         }
         if (gate_shared && --gate_left == 0) {
@@ -789,10 +881,10 @@ norm_residual_ring_kernel(const NormParams p, const RingPlan plan) {
 // BETA: sums for post_beta / pre_beta (and for a shared gate's share of post_beta) are kept.
 // Per task: s1 = sum D a hat(h), s0 = sum D a, with a = 1 where the gate is shared -- its factor, like the
 // block's scale, comes in when the task ends: dpost_gamma += scale a s1, dgate = scale act' (gamma s1 + beta s0).
-template <class T, int PACKS, bool BETA>
+template <class T, int PACKS, bool BETA, bool VEC>
 __global__ void __launch_bounds__(512, 1)
 norm_residual_backward_ring_kernel(const NormParams p, const RingPlan plan) {
-    constexpr int N = kPack<T>, M = N / 2;
+    constexpr int N = Columns<T, VEC>::N, M = N / 2;
     constexpr int MB = BETA ? M : 1;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ RingSums<2> sums;
@@ -800,16 +892,15 @@ norm_residual_backward_ring_kernel(const NormParams p, const RingPlan plan) {
     __shared__ alignas(16) float4 stat[kMaxStages];  // the rows' statistics, beside their stages
     RingTeam<2> team{&sums, 0, static_cast<int>(blockDim.x) / kWarp, static_cast<int>(cluster_size()),
                      static_cast<int>(cluster_rank())};
-    const int t = threadIdx.x, threads = blockDim.x;
-    const int row_packs = p.cols / N, slice = plan.slice_packs;
-    const int first = team.rank * slice;
-    const int count = min(slice, row_packs - first);
+    const int t = threadIdx.x;
+    const int units = VEC ? p.cols / kPack<T> : p.cols;
+    const Columns<T, VEC> own{t, static_cast<int>(blockDim.x), team.rank * plan.slice, min(plan.slice, units - team.rank * plan.slice)};
     const int64_t teams = gridDim.x / team.cluster, id = blockIdx.x / team.cluster;
     const bool gate_each = p.gate != nullptr && p.rows_per_gate == 1;
     const bool gate_shared = p.gate != nullptr && !gate_each;
-    uint4* const stages = reinterpret_cast<uint4*>(smem);  // [stages][tiles][slice]
-    float4* const w1 = reinterpret_cast<float4*>(stages + static_cast<size_t>(plan.stages) * plan.tiles * slice);
-    float4* const w2 = w1 + slice * (N / 4);
+    uint4* const stages = reinterpret_cast<uint4*>(smem);  // [stages][tiles][tile]
+    float* const w1 = reinterpret_cast<float*>(stages + static_cast<size_t>(plan.stages) * plan.tiles * plan.tile);
+    float* const w2 = w1 + plan.weights;
     // Places of the tensors in a stage; an absent one has none.
     const int at_dn = 0, at_y = 1;
     const int at_h = p.dn != nullptr ? 2 : 0;
@@ -834,19 +925,21 @@ norm_residual_backward_ring_kernel(const NormParams p, const RingPlan plan) {
     if (ask_task < p.tasks) task_rows(ask_task, &ask_row, &ask_end);
     auto request = [&](int stage) {
         if (ask_task >= p.tasks) return;
-        const size_t at = (static_cast<size_t>(ask_row) * p.cols + static_cast<size_t>(first) * N) * sizeof(T);
-        uint4* tile = stages + static_cast<size_t>(stage) * plan.tiles * slice;
+        const auto span = own.span(ask_row, p.cols, p.rows);
+        uint4* tile = stages + static_cast<size_t>(stage) * plan.tiles * plan.tile;
         uint64_t* bar = &full[stage];
-        const uint32_t bytes = static_cast<uint32_t>(count) * 16u;
-        mbar_expect_tx(bar, static_cast<uint32_t>(plan.tiles) * bytes + 16u);
+        mbar_expect_tx(bar, static_cast<uint32_t>(plan.tiles) * span.bytes + 16u);
         bulk_g2s(&stat[stage], p.stats_in + 4 * ask_row, 16u, bar);
+        auto ask = [&](int place, const void* tensor) {
+            bulk_g2s(tile + place * plan.tile, static_cast<const unsigned char*>(tensor) + span.from, span.bytes, bar);
+        };
         if (p.dn != nullptr) {
-            bulk_g2s(tile + at_dn * slice, static_cast<const unsigned char*>(p.dn) + at, bytes, bar);
-            bulk_g2s(tile + at_y * slice, static_cast<const unsigned char*>(p.y_in) + at, bytes, bar);
+            ask(at_dn, p.dn);
+            ask(at_y, p.y_in);
         }
-        bulk_g2s(tile + at_h * slice, static_cast<const unsigned char*>(p.h) + at, bytes, bar);
-        if (p.dy != nullptr) bulk_g2s(tile + at_dy * slice, static_cast<const unsigned char*>(p.dy) + at, bytes, bar);
-        if (gate_each) bulk_g2s(tile + at_gate * slice, static_cast<const unsigned char*>(p.gate) + at, bytes, bar);
+        ask(at_h, p.h);
+        if (p.dy != nullptr) ask(at_dy, p.dy);
+        if (gate_each) ask(at_gate, p.gate);
         if (++ask_row == ask_end) {
             ask_task += teams;
             if (ask_task < p.tasks) task_rows(ask_task, &ask_row, &ask_end);
@@ -858,20 +951,19 @@ norm_residual_backward_ring_kernel(const NormParams p, const RingPlan plan) {
     float2 s1[PACKS][M], s0[PACKS][MB], a2[PACKS][M], a3[PACKS][MB];
 #pragma unroll
     for (int k = 0; k < PACKS; ++k) {
-        const int i = t + k * threads;
 #pragma unroll
         for (int e = 0; e < M; ++e) {
             s1[k][e] = a2[k][e] = both(0.0f);
             s0[k][e % MB] = a3[k][e % MB] = both(0.0f);
         }
-        if (i < count) {
+        if (own.has(k)) {
             float2 w[M];
-            fetch_floats(p.post_gamma, (first + i) * N, w);
+            own.fetch(p.post_gamma, k, w);
 #pragma unroll
             for (int e = 0; e < M; ++e) w[e] = mul2(w[e], both(p.block_scale));
-            keep_floats(w1, i, slice, w);
-            fetch_floats(p.pre_gamma, (first + i) * N, w);
-            keep_floats(w2, i, slice, w);
+            own.keep(w1, k, w);
+            own.fetch(p.pre_gamma, k, w);
+            own.keep(w2, k, w);
         }
     }
     RingWait ring{full, plan.stages, 0, 0, false};
@@ -884,22 +976,25 @@ norm_residual_backward_ring_kernel(const NormParams p, const RingPlan plan) {
         if (gate_shared) {
 #pragma unroll
             for (int k = 0; k < PACKS; ++k) {
-                const int i = t + k * threads;
-                if (i >= count) continue;
+                if (!own.has(k)) continue;
                 float2 g[M], w[M];
-                unpack2(*reinterpret_cast<const uint4*>(static_cast<const T*>(p.gate) + group * p.cols + (first + i) * N), g, T{});
+                own.load_row(static_cast<const T*>(p.gate) + group * p.cols, k, g);
                 gate_pairs(p.gate_act, g);
-                fetch_floats(p.post_gamma, (first + i) * N, w);
+                own.fetch(p.post_gamma, k, w);
 #pragma unroll
                 for (int e = 0; e < M; ++e) w[e] = mul2(mul2(w[e], both(p.block_scale)), g[e]);
-                keep_floats(w1, i, slice, w);
+                own.keep(w1, k, w);
             }
         }
         for (int64_t row = from; row < to; ++row) {
             ring.wait(p.error_flag);
-            const uint4* tile = stages + static_cast<size_t>(ring.stage) * plan.tiles * slice;
+            const uint4* tile = stages + static_cast<size_t>(ring.stage) * plan.tiles * plan.tile;
             const float4 st = stat[ring.stage];
-            const int64_t base = row * p.cols + static_cast<int64_t>(first) * N;
+            const int64_t base = row * p.cols;
+            const auto span = own.span(row, p.cols, p.rows);
+            auto fetch = [&](int place, const void* tensor, int k, float2 (&v)[M]) {
+                own.load(tile + place * plan.tile, span, static_cast<const T*>(tensor) + base, k, v);
+            };
             float2 d[PACKS][M], hat[PACKS][M];
             float level = 0.0f, along = 0.0f;
             if (p.dn != nullptr) {
@@ -907,12 +1002,11 @@ norm_residual_backward_ring_kernel(const NormParams p, const RingPlan plan) {
                 const float2 r = both(st.w), shift = both(-st.z * st.w);
 #pragma unroll
                 for (int k = 0; k < PACKS; ++k) {
-                    const int i = t + k * threads;
-                    if (i < count) {
+                    if (own.has(k)) {
                         float2 w[M];
-                        unpack2(tile[at_dn * slice + i], d[k], T{});
-                        unpack2(tile[at_y * slice + i], hat[k], T{});
-                        load_floats(w2, i, slice, w);
+                        fetch(at_dn, p.dn, k, d[k]);
+                        fetch(at_y, p.y_in, k, hat[k]);
+                        own.kept(w2, k, w);
 #pragma unroll
                         for (int e = 0; e < M; ++e) {
                             hat[k][e] = fma2(hat[k][e], r, shift);
@@ -944,12 +1038,11 @@ norm_residual_backward_ring_kernel(const NormParams p, const RingPlan plan) {
                 const float2 down = both(-along), lower = both(-level);
 #pragma unroll
                 for (int k = 0; k < PACKS; ++k) {
-                    const int i = t + k * threads;
-                    if (i >= count) continue;
+                    if (!own.has(k)) continue;
                     float2 w[M];
                     // D, and dx
                     if (p.dy != nullptr) {
-                        unpack2(tile[at_dy * slice + i], w, T{});
+                        fetch(at_dy, p.dy, k, w);
 #pragma unroll
                         for (int e = 0; e < M; ++e) d[k][e] = fma2(r2, fma2(hat[k][e], down, add2(d[k][e], lower)), w[e]);
                     } else {
@@ -959,20 +1052,20 @@ norm_residual_backward_ring_kernel(const NormParams p, const RingPlan plan) {
                     if (p.dx != nullptr) {
 #pragma unroll
                         for (int e = 0; e < M; ++e) w[e] = mul2(both(p.residual_scale), d[k][e]);
-                        store_pairs(static_cast<T*>(p.dx) + base + static_cast<int64_t>(i) * N, w);
+                        own.store(static_cast<T*>(p.dx) + base, k, w);
                     }
-                    unpack2(tile[at_h * slice + i], hat[k], T{});
+                    fetch(at_h, p.h, k, hat[k]);
 #pragma unroll
                     for (int e = 0; e < M; ++e) hat[k][e] = fma2(hat[k][e], r1, shift);
                     float2 scale[M];
-                    load_floats(w1, i, slice, scale);  // block_scale * gamma (* a shared gate)
+                    own.kept(w1, k, scale);  // block_scale * gamma (* a shared gate)
                     if (gate_each) {
                         float2 a[M];
-                        unpack2(tile[at_gate * slice + i], a, T{});
+                        fetch(at_gate, p.gate, k, a);
                         gate_pairs(p.gate_act, a);
                         if (p.dgate != nullptr) {
                             if (BETA && p.post_beta != nullptr) {
-                                fetch_floats(p.post_beta, (first + i) * N, w);
+                                own.fetch(p.post_beta, k, w);
 #pragma unroll
                                 for (int e = 0; e < M; ++e) w[e] = mul2(d[k][e], fma2(hat[k][e], scale[e], mul2(both(p.block_scale), w[e])));
                             } else {
@@ -980,7 +1073,7 @@ norm_residual_backward_ring_kernel(const NormParams p, const RingPlan plan) {
                                 for (int e = 0; e < M; ++e) w[e] = mul2(d[k][e], mul2(hat[k][e], scale[e]));
                             }
                             times_slope_pairs(p.gate_act, a, w);
-                            store_pairs(static_cast<T*>(p.dgate) + base + static_cast<int64_t>(i) * N, w);
+                            own.store(static_cast<T*>(p.dgate) + base, k, w);
                         }
 #pragma unroll
                         for (int e = 0; e < M; ++e) d[k][e] = mul2(d[k][e], a[e]);
@@ -1004,11 +1097,10 @@ norm_residual_backward_ring_kernel(const NormParams p, const RingPlan plan) {
                 const float2 r1 = both(st.y), down = both(-along), lower = both(-level);
 #pragma unroll
                 for (int k = 0; k < PACKS; ++k) {
-                    const int i = t + k * threads;
-                    if (i >= count) continue;
+                    if (!own.has(k)) continue;
 #pragma unroll
                     for (int e = 0; e < M; ++e) d[k][e] = mul2(r1, fma2(hat[k][e], down, add2(d[k][e], lower)));
-                    store_pairs(static_cast<T*>(p.dh) + base + static_cast<int64_t>(i) * N, d[k]);
+                    own.store(static_cast<T*>(p.dh) + base, k, d[k]);
                 }
             }
             ring.next();
@@ -1018,56 +1110,59 @@ norm_residual_backward_ring_kernel(const NormParams p, const RingPlan plan) {
         if (!gate_shared && !last) continue;
 #pragma unroll
         for (int k = 0; k < PACKS; ++k) {
-            const int i = t + k * threads;
-            if (i >= count) continue;
-            float g[N], a[N];
+            if (!own.has(k)) continue;
+            float2 g[M], a[M];
             if (gate_shared) {
-                Chunk<T, N>::load(static_cast<const T*>(p.gate) + group * p.cols + (first + i) * N, a);
-                gate_values(p.gate_act, a);
+                own.load_row(static_cast<const T*>(p.gate) + group * p.cols, k, a);
+                gate_pairs(p.gate_act, a);
             } else {
 #pragma unroll
-                for (int e = 0; e < N; ++e) a[e] = 1.0f;
+                for (int e = 0; e < M; ++e) a[e] = both(1.0f);
+            }
+#pragma unroll
+            for (int e = 0; e < M; ++e) g[e] = both(0.0f);
+            if (gate_shared && p.dgate != nullptr) {
+                own.fetch(p.post_gamma, k, g);
+#pragma unroll
+                for (int e = 0; e < M; ++e) g[e] = mul2(g[e], s1[k][e]);
+                if (BETA && p.post_beta != nullptr) {
+                    float2 b[M];
+                    own.fetch(p.post_beta, k, b);
+#pragma unroll
+                    for (int e = 0; e < M; ++e) g[e] = fma2(b[e], s0[k][e % MB], g[e]);
+                }
+#pragma unroll
+                for (int e = 0; e < M; ++e) g[e] = mul2(g[e], both(p.block_scale));
+                times_slope_pairs(p.gate_act, a, g);
+                if (p.gate_partial == nullptr) own.store(static_cast<T*>(p.dgate) + group * p.cols, k, g);
             }
 #pragma unroll
             for (int e = 0; e < N; ++e) {
-                const int c = (first + i) * N + e;
-                const float f = e % 2 == 0 ? s1[k][e / 2].x : s1[k][e / 2].y;
-                const float b = !BETA ? 0.0f : e % 2 == 0 ? s0[k][e / 2 % MB].x : s0[k][e / 2 % MB].y;
-                g[e] = 0.0f;
-                if (gate_shared && p.dgate != nullptr) {
-                    float u = (p.post_gamma != nullptr ? p.post_gamma[c] : 1.0f) * f;
-                    if (BETA && p.post_beta != nullptr) u += p.post_beta[c] * b;
-                    g[e] = p.block_scale * u;
-                }
+                if (!own.inside(e)) continue;
+                const int c = own.col(k, e);
+                const float f = (e % 2 == 0 ? s1[k][e / 2].x * a[e / 2].x : s1[k][e / 2].y * a[e / 2].y) * p.block_scale;
+                const float b = !BETA ? 0.0f : (e % 2 == 0 ? s0[k][e / 2 % MB].x * a[e / 2].x : s0[k][e / 2 % MB].y * a[e / 2].y) * p.block_scale;
                 float* const pg = p.partial[0] != nullptr ? p.partial[0] + id * p.cols + c : nullptr;
                 float* const pb = p.partial[1] != nullptr ? p.partial[1] + id * p.cols + c : nullptr;
-                if (pg != nullptr) *pg = (flushed ? *pg : 0.0f) + p.block_scale * a[e] * f;
-                if (pb != nullptr) *pb = (flushed ? *pb : 0.0f) + p.block_scale * a[e] * b;
+                if (pg != nullptr) *pg = (flushed ? *pg : 0.0f) + f;
+                if (pb != nullptr) *pb = (flushed ? *pb : 0.0f) + b;
+                if (gate_shared && p.gate_partial != nullptr) p.gate_partial[task * p.cols + c] = e % 2 == 0 ? g[e / 2].x : g[e / 2].y;
             }
 #pragma unroll
             for (int e = 0; e < M; ++e) {
                 s1[k][e] = both(0.0f);
                 if (BETA) s0[k][e % MB] = both(0.0f);
             }
-            times_slope(p.gate_act, a, g);
-            if (gate_shared && p.dgate != nullptr) {
-                if (p.gate_partial != nullptr) {
-#pragma unroll
-                    for (int e = 0; e < N; ++e) p.gate_partial[task * p.cols + (first + i) * N + e] = g[e];
-                } else {
-                    Chunk<T, N>::store_stream(static_cast<T*>(p.dgate) + group * p.cols + (first + i) * N, g);
-                }
-            }
         }
         flushed = true;
     }
 #pragma unroll
     for (int k = 0; k < PACKS; ++k) {
-        const int i = t + k * threads;
-        if (i >= count) continue;
+        if (!own.has(k)) continue;
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-            const int64_t c = id * p.cols + (first + i) * N + e;
+            if (!own.inside(e)) continue;
+            const int64_t c = id * p.cols + own.col(k, e);
             if (p.partial[2] != nullptr) p.partial[2][c] = e % 2 == 0 ? a2[k][e / 2].x : a2[k][e / 2].y;
             if (BETA && p.partial[3] != nullptr) p.partial[3][c] = e % 2 == 0 ? a3[k][e / 2 % MB].x : a3[k][e / 2 % MB].y;
             if (!flushed) {  // a team without a task
@@ -1144,28 +1239,38 @@ Shape shape_of(int64_t cols) {
 // The ring form: columns of a CTA, its threads and its stages; stages == 0: does not fit.
 struct RingShape {
     int threads, cluster, blocks, per_thread;  // CTAs a row, CTAs an SM, columns a thread
+    bool vec;                                  // whole packs a row
     RingPlan plan;
     size_t smem;
 };
 
 // A thread owns 8 columns, or 16 of a 16-bit type (two packs: the sums' instructions are shared by more
-// columns) -- but not for sums for the betas, whose registers would spill.  Stages take what is left of the
-// shared memory of an SM, shared by as many CTAs as 1024 threads make (backward: 512, with 128 registers each).
+// columns) -- but not for sums for the betas, whose registers would spill, nor where columns go one by one.  Stages
+// take what is left of the shared memory of an SM, shared by as many CTAs as 1024 threads make (backward: 512,
+// with 128 registers each).
 RingShape ring_shape(int64_t cols, int dtype, int tiles, int weights, bool backward, bool beta) {
     RingShape r = {};
-    const int n = 16 / static_cast<int>(dtype_bytes(dtype));
-    if (cols % n != 0 || cols <= kWarpCols) return r;  // no whole packs, or a warp a row
-    const int64_t packs = cols / n;
-    r.per_thread = dtype != FDL_F32 && !beta ? 16 : 8;
+    const int size = static_cast<int>(dtype_bytes(dtype)), n = 16 / size;
+    if (cols <= kWarpCols) return r;  // a warp a row
+    r.vec = cols % n == 0;
+    r.per_thread = r.vec && dtype != FDL_F32 && !beta ? 16 : 8;
     r.cluster = 1;
     while (cols > static_cast<int64_t>(r.cluster) * 512 * r.per_thread) r.cluster *= 2;
-    r.plan.slice_packs = static_cast<int>(ceil_div(packs, r.cluster));
     r.plan.tiles = tiles;
-    r.threads = static_cast<int>(ceil_div(ceil_div(r.plan.slice_packs, r.per_thread / n), kWarp)) * kWarp;
+    if (r.vec) {
+        r.plan.slice = r.plan.tile = static_cast<int>(ceil_div(cols / n, r.cluster));
+        r.threads = static_cast<int>(ceil_div(ceil_div(r.plan.slice, r.per_thread / n), kWarp)) * kWarp;
+        r.plan.weights = r.plan.slice * n;
+    } else {
+        r.plan.slice = static_cast<int>(ceil_div(cols, r.cluster));
+        r.plan.tile = (r.plan.slice * size + 30) / 16;  // any 16-byte words that cover the columns
+        r.threads = static_cast<int>(ceil_div(ceil_div(r.plan.slice, r.per_thread), kWarp)) * kWarp;
+        r.plan.weights = r.threads * 8;
+    }
     const int budget = backward ? 512 : 1024;
     r.blocks = budget / r.threads < 1 ? 1 : budget / r.threads > 16 ? 16 : budget / r.threads;
-    const size_t fixed = static_cast<size_t>(r.plan.slice_packs) * n * 4 * weights;
-    const size_t stage = static_cast<size_t>(r.plan.slice_packs) * 16 * tiles;
+    const size_t fixed = static_cast<size_t>(r.plan.weights) * 4 * weights;
+    const size_t stage = static_cast<size_t>(r.plan.tile) * 16 * tiles;
     for (; r.blocks >= 1; --r.blocks) {  // fewer CTAs where less than two stages would fit
         const size_t room = static_cast<size_t>(227 * 1024) / r.blocks - 4096;
         if (room < fixed + 2 * stage) continue;
@@ -1284,16 +1389,34 @@ int launch_ring(K kernel, const NormParams& p, const RingShape& r, int64_t grid,
 int launch_ring_forward(int dtype, const NormParams& p, const RingShape& r, int64_t grid, cudaStream_t stream) {
     return with_dtype(dtype, [&](auto* tag) {
         using T = std::remove_pointer_t<decltype(tag)>;
-        return launch_ring(norm_residual_ring_kernel<T, 2>, p, r, grid, stream);
+        return r.vec ? launch_ring(norm_residual_ring_kernel<T, 2, true>, p, r, grid, stream)
+                     : launch_ring(norm_residual_ring_kernel<T, 1, false>, p, r, grid, stream);
     });
 }
 
 int launch_ring_backward(int dtype, bool beta, const NormParams& p, const RingShape& r, int64_t grid, cudaStream_t stream) {
     return with_dtype(dtype, [&](auto* tag) {
         using T = std::remove_pointer_t<decltype(tag)>;
-        return beta ? launch_ring(norm_residual_backward_ring_kernel<T, 8 / kPack<T>, true>, p, r, grid, stream)
-                    : launch_ring(norm_residual_backward_ring_kernel<T, 2, false>, p, r, grid, stream);
+        if (!r.vec) {
+            return beta ? launch_ring(norm_residual_backward_ring_kernel<T, 1, true, false>, p, r, grid, stream)
+                        : launch_ring(norm_residual_backward_ring_kernel<T, 1, false, false>, p, r, grid, stream);
+        }
+        return beta ? launch_ring(norm_residual_backward_ring_kernel<T, 8 / kPack<T>, true, true>, p, r, grid, stream)
+                    : launch_ring(norm_residual_backward_ring_kernel<T, 2, false, true>, p, r, grid, stream);
     });
+}
+
+// Whether the ring form can take its tensors: those that it copies start on the 16-byte grid, and with whole packs a
+// row so does everything else (`others`).
+bool ring_fits(const RingShape& r, std::initializer_list<const void*> copied, std::initializer_list<const void*> others) {
+    if (r.plan.stages < 2) return false;
+    for (const void* t : copied) {
+        if (!aligned16(t)) return false;
+    }
+    for (const void* t : others) {
+        if (r.vec && !aligned16(t)) return false;
+    }
+    return true;
 }
 
 }  // namespace
@@ -1331,10 +1454,10 @@ int fdl_norm_residual(const void* x, const void* h, const void* gate, int64_t ga
     p.residual_scale = residual_scale; p.block_scale = block_scale; p.eps = eps;
     const bool vec = packs_fit(dtype, cols, {x, h, gate, y, n});
     const Shape s = shape_of(cols);
-    if (vec && aligned16(post_gamma) && aligned16(post_beta) && aligned16(pre_gamma) && aligned16(pre_beta)) {
-        const RingShape r = ring_shape(cols, dtype, 2 + (gate != nullptr && gate_rows == rows), 0, false, false);
-        const int64_t teams = r.plan.stages >= 2 ? static_cast<int64_t>(info->sm_count) * r.blocks / r.cluster : rows;
-        if (rows > teams) {
+    const RingShape r = ring_shape(cols, dtype, 2 + (gate != nullptr && gate_rows == rows), 0, false, false);
+    if (ring_fits(r, {x, h, gate}, {y, n, post_gamma, post_beta, pre_gamma, pre_beta})) {
+        const int64_t teams = static_cast<int64_t>(info->sm_count) * r.blocks / r.cluster;
+        if (rows > teams) {  // (for one row a team the copies ahead have nothing to run ahead of)
             status = error_flag_device_ptr(&p.error_flag);
             if (status != FDL_OK) return status;
             return launch_ring_forward(dtype, p, r, teams * r.cluster, as_stream(stream));
@@ -1415,7 +1538,7 @@ int fdl_norm_residual_backward(const void* dy, const void* dn, const void* y, co
     const bool beta = dpost_beta != nullptr || dpre_beta != nullptr || (post_beta != nullptr && dgate != nullptr);
     const int tiles = 1 + (dn != nullptr ? 2 : 0) + (dy != nullptr) + (gate != nullptr && gate_rows == rows);
     const RingShape r = ring_shape(cols, dtype, tiles, 2, true, beta);
-    const bool ring = vec && r.plan.stages >= 2 && aligned16(post_gamma) && aligned16(post_beta) && aligned16(pre_gamma);
+    const bool ring = ring_fits(r, {dy, dn, y, h, gate}, {dx, dh, dgate, post_gamma, post_beta, pre_gamma});
     const BackwardPlan b = backward_plan(rows, cols, gate_rows, info->sm_count, ring ? &r : nullptr);
     NormParams p = {};
     p.dy = dy; p.dn = dn; p.y_in = y; p.h = h; p.stats_in = stats; p.gate = gate;

@@ -252,9 +252,10 @@ def test_many_rows_and_their_gates(fdl, cuda, rows, gates, cols):
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("rows,cols,gates", [(1400, 264, 7), (2500, 512, 1), (601, 1000, 601), (700, 2048, 0), (450, 4096, 450),
                                              (450, 4096, 150), (330, 4104, 3), (400, 8192, 2), (151, 8200, 1), (160, 16384, 160),
-                                             (90, 32768, 9)])
+                                             (90, 32768, 9), (1500, 257, 3), (1201, 330, 1201), (500, 1001, 0), (600, 2049, 2), (301, 4095, 301),
+                                             (170, 5003, 10), (160, 9001, 1), (75, 30001, 75)])
 def test_more_rows_than_teams(fdl, cuda, rows, cols, gates, kind):
-    """Whole packs a row, and several rows for each team, from one to eight CTAs wide."""
+    """Several rows for each team, from one to eight CTAs wide, rows of whole packs and rows off the 16-byte grid."""
     check(fdl, Case(rows, cols, kind, RMS, RMS, gates, SIGMOID if gates else PLAIN).cuda(), ("both", "dn"))
     check(fdl, Case(rows, cols, kind, LAYER, LAYER, gates, TANH if gates else PLAIN, seed=2).cuda(), ("both", "dy"))
     check(fdl, Case(rows, cols, kind, NONE, NONE, gates, PLAIN).cuda())
