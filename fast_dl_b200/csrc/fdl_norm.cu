@@ -540,19 +540,61 @@ struct RingPlan {
 template <int NV>
 struct RingSums {
     alignas(16) float buf[2][kMaxCluster * kMaxWarps * NV];
+    uint64_t full[2];  // clusters: a buffer's values have arrived
 };
+
+// A store into CTA `rank`'s copy of `mine`, counted on its copy of `bar`.  A cluster barrier in its place would wait
+// for the rows' gradient stores, a microsecond or two at each of a row's sums.  (Launches with clusters only.)
+template <int NV>
+__device__ __forceinline__ void send(float* mine, uint64_t* bar, uint32_t rank, const float (&v)[NV]) {
+    uint32_t to, at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_addr(mine)), "r"(rank));
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_addr(bar)), "r"(rank));
+    if constexpr (NV == 2) {
+        asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(to), "f"(v[0]),
+                     "f"(v[1]), "r"(at)
+                     : "memory");
+    } else {
+        asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.f32 [%0], %1, [%2];" ::"r"(to), "f"(v[0]), "r"(at)
+                     : "memory");
+    }
+}
+__device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(smem_addr(bar)), "r"(parity)
+        : "memory");
+    return done != 0;
+}
 
 template <int NV>
 struct RingTeam {
     RingSums<NV>* sums;
     int phase, warps, cluster, rank;
-    // NV sums over the row's team: one barrier, alternating buffers.
+    uint32_t parity;  // bit i: of buffer i's next round
+    bool failed;
+    unsigned int* error_flag;
+
+    __device__ __forceinline__ RingTeam(RingSums<NV>* s, unsigned int* flag)
+        : sums(s), phase(0), warps(blockDim.x / kWarp), cluster(cluster_size()), rank(cluster_rank()), parity(0), failed(false),
+          error_flag(flag) {
+        if (threadIdx.x == 0) {
+            mbar_init(&sums->full[0], 1);
+            mbar_init(&sums->full[1], 1);
+        }
+    }
+    // NV sums over the row's team; the buffers alternate.  A buffer's next values are sent when everybody has sent
+    // those of the other one, and so has read it.
     __device__ __forceinline__ void sum(float (&v)[NV]) {
         const int lane = threadIdx.x & (kWarp - 1), warp = threadIdx.x / kWarp;
 #pragma unroll
         for (int i = 0; i < NV; ++i) v[i] = warp_sum(v[i]);
         float* at = sums->buf[phase];
-        phase ^= 1;
+        const int n = warps * cluster;
         if (cluster == 1) {
             if (lane == 0) {
 #pragma unroll
@@ -560,14 +602,19 @@ struct RingTeam {
             }
             __syncthreads();
         } else {
-            if (lane < cluster) {
-#pragma unroll
-                for (int i = 0; i < NV; ++i) store_remote(&at[(rank * warps + warp) * NV + i], lane, v[i]);
+            uint64_t* bar = &sums->full[phase];
+            if (threadIdx.x == 0) mbar_expect_tx(bar, static_cast<uint32_t>(n * NV * sizeof(float)));
+            if (lane < cluster) send(&at[(rank * warps + warp) * NV], bar, lane, v);
+            bool ok = failed;  // after a wait that ran out there is no more waiting
+            for (uint32_t i = 0; i < kMbarSpinLimit && !ok; ++i) ok = mbar_try_wait_cluster(bar, parity >> phase & 1u);
+            if (!ok) {
+                failed = true;
+                atomicOr_system(error_flag, 1u);
             }
-            cluster_sync_all();
+            parity ^= 1u << phase;
         }
+        phase ^= 1;
         // Each warp folds the partial sums by itself, all in the same order.
-        const int n = warps * cluster;
 #pragma unroll
         for (int i = 0; i < NV; ++i) v[i] = lane < n ? at[lane * NV + i] : 0.0f;
         for (int w = lane + kWarp; w < n; w += kWarp) {
@@ -724,8 +771,7 @@ norm_residual_ring_kernel(const NormParams p, const RingPlan plan) {
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ RingSums<1> sums;
     __shared__ uint64_t full[kMaxStages];
-    RingTeam<1> team{&sums, 0, static_cast<int>(blockDim.x) / kWarp, static_cast<int>(cluster_size()),
-                     static_cast<int>(cluster_rank())};
+    RingTeam<1> team(&sums, p.error_flag);
     const int t = threadIdx.x;
     const int units = VEC ? p.cols / kPack<T> : p.cols;
     const Columns<T, VEC> own{t, static_cast<int>(blockDim.x), team.rank * plan.slice, min(plan.slice, units - team.rank * plan.slice)};
@@ -890,8 +936,7 @@ norm_residual_backward_ring_kernel(const NormParams p, const RingPlan plan) {
     __shared__ RingSums<2> sums;
     __shared__ uint64_t full[kMaxStages];
     __shared__ alignas(16) float4 stat[kMaxStages];  // the rows' statistics, beside their stages
-    RingTeam<2> team{&sums, 0, static_cast<int>(blockDim.x) / kWarp, static_cast<int>(cluster_size()),
-                     static_cast<int>(cluster_rank())};
+    RingTeam<2> team(&sums, p.error_flag);
     const int t = threadIdx.x;
     const int units = VEC ? p.cols / kPack<T> : p.cols;
     const Columns<T, VEC> own{t, static_cast<int>(blockDim.x), team.rank * plan.slice, min(plan.slice, units - team.rank * plan.slice)};
@@ -1186,26 +1231,27 @@ struct FoldJobs {
     int cols;
 };
 
-constexpr int kFoldX = 32, kFoldY = 16;
+// 32 columns a CTA, blockDim.y strands of rows each: eight loads of a strand are on their way at a time, so the host
+// takes more strands for more rows.
+constexpr int kFoldX = 32, kFoldY = 32;
 
 __global__ void __launch_bounds__(kFoldX * kFoldY)
 norm_fold_kernel(const FoldJobs jobs) {
     __shared__ float red[kFoldY][kFoldX + 1];
     const FoldJob job = jobs.job[blockIdx.y];
-    const int c = blockIdx.x * kFoldX + threadIdx.x;
+    const int c = blockIdx.x * kFoldX + threadIdx.x, strands = blockDim.y;
     pdl_wait();
     for (int64_t g = blockIdx.z; g < job.groups; g += gridDim.z) {
         float s = 0.0f;
         if (c < jobs.cols) {
-#pragma unroll 4
-            for (int64_t r = threadIdx.y; r < job.each; r += kFoldY) s += job.part[(g * job.each + r) * jobs.cols + c];
+#pragma unroll 8
+            for (int64_t r = threadIdx.y; r < job.each; r += strands) s += job.part[(g * job.each + r) * jobs.cols + c];
         }
         red[threadIdx.y][threadIdx.x] = s;
         __syncthreads();
         if (threadIdx.y == 0 && c < jobs.cols) {
             s = red[0][threadIdx.x];
-#pragma unroll
-            for (int k = 1; k < kFoldY; ++k) s += red[k][threadIdx.x];
+            for (int k = 1; k < strands; ++k) s += red[k][threadIdx.x];
             const int64_t at = g * jobs.cols + c;
             if (job.dtype == FDL_F32) static_cast<float*>(job.out)[at] = s;
             else if (job.dtype == FDL_F16) static_cast<__half*>(job.out)[at] = from_f32<__half>(s);
@@ -1577,7 +1623,8 @@ int fdl_norm_residual_backward(const void* dy, const void* dn, const void* y, co
     if (status != FDL_OK || njobs == 0) return status;
     const dim3 grid(static_cast<unsigned int>(ceil_div(cols, kFoldX)), static_cast<unsigned int>(njobs),
                     static_cast<unsigned int>(groups < 64 ? groups : 64));
-    return launch_ex(norm_fold_kernel, grid, dim3(kFoldX, kFoldY), 0, s, dim3(1, 1, 1), tuning().pdl != 0, jobs);
+    const int strands = b.teams <= 64 ? 4 : b.teams <= 256 ? 8 : b.teams <= 512 ? 16 : kFoldY;
+    return launch_ex(norm_fold_kernel, grid, dim3(kFoldX, strands), 0, s, dim3(1, 1, 1), tuning().pdl != 0, jobs);
 }
 
 }  // extern "C"
