@@ -94,14 +94,12 @@ struct TeamSums {
     float2 buf[2][kMaxCluster * kMaxWarps];
 };
 
-template <bool WARP>
 struct Team {
     TeamSums* sums;
     int phase, warps, cluster, rank;
     __device__ __forceinline__ float2 sum(float a, float b) {
         a = warp_sum(a);
         b = warp_sum(b);
-        if (WARP) return make_float2(a, b);
         const int lane = threadIdx.x & (kWarp - 1), warp = threadIdx.x / kWarp;
         float2* at = sums->buf[phase];
         phase ^= 1;
@@ -238,30 +236,17 @@ __device__ __forceinline__ float2 moments(int kind, float eps, const float (&v)[
     return make_float2(mean, 1.0f / sqrtf(var + eps));
 }
 
-template <class T, int N, int PACKS, bool WARP>
+template <class T, int N, int PACKS>
 __global__ void __launch_bounds__(512)
 norm_residual_kernel(const NormParams p) {
     __shared__ TeamSums sums;
-    Team<WARP> team{&sums, 0, static_cast<int>(blockDim.x) / kWarp, 1, 0};
+    Team team{&sums, 0, static_cast<int>(blockDim.x) / kWarp, static_cast<int>(cluster_size()), static_cast<int>(cluster_rank())};
     Owned<N, PACKS> own;
-    int64_t row, step;
-    if (WARP) {
-        const int warps = blockDim.x / kWarp;
-        own.first = threadIdx.x & (kWarp - 1);
-        own.stride = kWarp;
-        row = static_cast<int64_t>(blockIdx.x) * warps + threadIdx.x / kWarp;
-        step = static_cast<int64_t>(gridDim.x) * warps;
-    } else {
-        team.cluster = static_cast<int>(cluster_size());
-        team.rank = static_cast<int>(cluster_rank());
-        own.first = team.rank * blockDim.x + threadIdx.x;
-        own.stride = team.cluster * blockDim.x;
-        row = blockIdx.x / team.cluster;
-        step = gridDim.x / team.cluster;
-        if (team.cluster > 1) cluster_sync_all();  // every CTA has started before the first remote store
-    }
+    own.first = team.rank * blockDim.x + threadIdx.x;
+    own.stride = team.cluster * blockDim.x;
+    if (team.cluster > 1) cluster_sync_all();  // every CTA has started before the first remote store
     pdl_wait();
-    for (; row < p.rows; row += step) {
+    for (int64_t row = blockIdx.x / team.cluster; row < p.rows; row += gridDim.x / team.cluster) {
         float h[PACKS][N], x[PACKS][N], w[PACKS][N];
         const int64_t base = row * p.cols;
         load_row<T>(static_cast<const T*>(p.h) + base, own, p.cols, h);
@@ -319,32 +304,20 @@ norm_residual_kernel(const NormParams p) {
             }
         }
     }
-    if (!WARP && team.cluster > 1) cluster_sync_all();  // no CTA leaves while another may still write its sums
+    if (team.cluster > 1) cluster_sync_all();  // no CTA leaves while another may still write its sums
 }
 
 // A team takes whole tasks: rows_per_task consecutive rows of one gate row.
-template <class T, int N, int PACKS, bool WARP>
+template <class T, int N, int PACKS>
 __global__ void __launch_bounds__(512)
 norm_residual_backward_kernel(const NormParams p) {
     __shared__ TeamSums sums;
-    Team<WARP> team{&sums, 0, static_cast<int>(blockDim.x) / kWarp, 1, 0};
+    Team team{&sums, 0, static_cast<int>(blockDim.x) / kWarp, static_cast<int>(cluster_size()), static_cast<int>(cluster_rank())};
     Owned<N, PACKS> own;
-    int64_t id, teams;
-    if (WARP) {
-        const int warps = blockDim.x / kWarp;
-        own.first = threadIdx.x & (kWarp - 1);
-        own.stride = kWarp;
-        id = static_cast<int64_t>(blockIdx.x) * warps + threadIdx.x / kWarp;
-        teams = static_cast<int64_t>(gridDim.x) * warps;
-    } else {
-        team.cluster = static_cast<int>(cluster_size());
-        team.rank = static_cast<int>(cluster_rank());
-        own.first = team.rank * blockDim.x + threadIdx.x;
-        own.stride = team.cluster * blockDim.x;
-        id = blockIdx.x / team.cluster;
-        teams = gridDim.x / team.cluster;
-        if (team.cluster > 1) cluster_sync_all();  // every CTA has started before the first remote store
-    }
+    own.first = team.rank * blockDim.x + threadIdx.x;
+    own.stride = team.cluster * blockDim.x;
+    const int64_t id = blockIdx.x / team.cluster, teams = gridDim.x / team.cluster;
+    if (team.cluster > 1) cluster_sync_all();  // every CTA has started before the first remote store
     pdl_wait();
     float acc[4][PACKS][N];
 #pragma unroll
@@ -515,7 +488,7 @@ norm_residual_backward_kernel(const NormParams p) {
             for (int e = 0; e < N; ++e) p.partial[a][id * p.cols + own.col(k) + e] = acc[a][k][e];
         }
     }
-    if (!WARP && team.cluster > 1) cluster_sync_all();  // no CTA leaves while another may still write its sums
+    if (team.cluster > 1) cluster_sync_all();  // no CTA leaves while another may still write its sums
 }
 
 // ---- rows through shared memory ------------------------------------------------------------------
@@ -709,6 +682,18 @@ struct Columns {
             for (int e = 0; e < M; ++e) v[e] = make_float2(f[2 * e], f[2 * e + 1]);
         }
     }
+    // The same from a tensor that the kernel may be writing in place, with 0 outside the row.
+    __device__ __forceinline__ void stream(const T* row, int k, float2 (&v)[M]) const {
+        if constexpr (VEC) {
+            unpack2(has(k) ? __ldcs(reinterpret_cast<const uint4*>(row + col(k, 0))) : make_uint4(0, 0, 0, 0), v, T{});
+        } else {
+            float f[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) f[e] = inside(e) ? to_f32(__ldcs(row + col(k, e))) : 0.0f;
+#pragma unroll
+            for (int e = 0; e < M; ++e) v[e] = make_float2(f[2 * e], f[2 * e + 1]);
+        }
+    }
     __device__ __forceinline__ void store(T* row, int k, const float2 (&v)[M]) const {
         if constexpr (VEC) {
             store_pairs(row + col(k, 0), v);
@@ -763,6 +748,304 @@ struct Columns {
         }
     }
 };
+
+// ---- short rows: a part of a warp a row ---------------------------------------------------------------
+//
+// Rows of up to 256 columns: TEAM lanes a row, 8 columns a lane, 32 / TEAM rows a warp side by side, sums by
+// shuffles alone.  The loops have the same length in all lanes of a warp; a team without a row works on the last
+// one and stores nothing.
+
+template <int TEAM>
+__device__ __forceinline__ float team_sum(float v) {
+#pragma unroll
+    for (int o = TEAM / 2; o > 0; o >>= 1) v += __shfl_xor_sync(kFullMask, v, o);
+    return v;
+}
+
+template <int TEAM, class Own, int PACKS, int M>
+__device__ __forceinline__ float2 team_moments(int kind, float eps, float inv, const float2 (&v)[PACKS][M], const Own& own) {
+    if (kind == FDL_NORM_NONE) return make_float2(0.0f, 1.0f);
+    float mean = 0.0f;
+    if (kind == FDL_NORM_LAYER) {
+        float2 s = both(0.0f);
+#pragma unroll
+        for (int k = 0; k < PACKS; ++k) {
+#pragma unroll
+            for (int e = 0; e < M; ++e) s = add2(s, v[k][e]);
+        }
+        mean = team_sum<TEAM>(s.x + s.y) * inv;
+    }
+    float2 q = both(0.0f);
+#pragma unroll
+    for (int k = 0; k < PACKS; ++k) {
+#pragma unroll
+        for (int e = 0; e < M; ++e) {
+            float2 c = add2(v[k][e], both(-mean));
+            if (!own.has(k) || !own.inside(2 * e)) c.x = 0.0f;
+            if (!own.has(k) || !own.inside(2 * e + 1)) c.y = 0.0f;
+            q = fma2(c, c, q);
+        }
+    }
+    return make_float2(mean, rsqrtf(fmaf(team_sum<TEAM>(q.x + q.y), inv, eps)));
+}
+
+constexpr int kTeamThreads = 256;
+
+template <class T, int PACKS, bool VEC, int TEAM>
+__global__ void __launch_bounds__(kTeamThreads, 4)
+norm_residual_team_kernel(const NormParams p) {
+    constexpr int M = Columns<T, VEC>::M;
+    const int t = threadIdx.x % TEAM;
+    const Columns<T, VEC> own{t, TEAM, 0, VEC ? p.cols / kPack<T> : p.cols};
+    const float inv = 1.0f / static_cast<float>(p.cols);
+    pdl_wait();
+    const int64_t step = static_cast<int64_t>(gridDim.x) * (kTeamThreads / TEAM);
+    int64_t row = static_cast<int64_t>(blockIdx.x) * (kTeamThreads / TEAM) + threadIdx.x / TEAM;
+    for (int64_t first = row - threadIdx.x % kWarp / TEAM; first < p.rows; first += step, row += step) {
+        const bool active = row < p.rows;
+        const int64_t at = active ? row : p.rows - 1, base = at * p.cols;
+        float2 v[PACKS][M], x[PACKS][M], w[M];
+#pragma unroll
+        for (int k = 0; k < PACKS; ++k) {
+            own.stream(static_cast<const T*>(p.h) + base, k, v[k]);
+            own.stream(static_cast<const T*>(p.x) + base, k, x[k]);
+        }
+        const float2 s1 = team_moments<TEAM>(p.post_kind, p.eps, inv, v, own);
+        const float2 r1 = both(s1.y * p.block_scale), shift1 = both(-s1.x * s1.y * p.block_scale);
+#pragma unroll
+        for (int k = 0; k < PACKS; ++k) {
+            if (!own.has(k)) continue;
+#pragma unroll
+            for (int e = 0; e < M; ++e) v[k][e] = fma2(v[k][e], r1, shift1);
+            if (p.post_gamma != nullptr) {
+                own.fetch(p.post_gamma, k, w);
+#pragma unroll
+                for (int e = 0; e < M; ++e) v[k][e] = mul2(v[k][e], w[e]);
+            }
+            if (p.post_beta != nullptr) {
+                own.fetch(p.post_beta, k, w);
+#pragma unroll
+                for (int e = 0; e < M; ++e) v[k][e] = fma2(both(p.block_scale), w[e], v[k][e]);
+            }
+            if (p.gate != nullptr) {
+                own.stream(static_cast<const T*>(p.gate) + (p.rows_per_gate == 1 ? at : at / p.rows_per_gate) * p.cols, k, w);
+                gate_pairs(p.gate_act, w);
+#pragma unroll
+                for (int e = 0; e < M; ++e) v[k][e] = mul2(v[k][e], w[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < M; ++e) {
+                v[k][e] = fma2(both(p.residual_scale), x[k][e], v[k][e]);
+                if (!own.inside(2 * e)) v[k][e].x = 0.0f;
+                if (!own.inside(2 * e + 1)) v[k][e].y = 0.0f;
+            }
+            if (active) own.store(static_cast<T*>(p.y) + base, k, v[k]);
+        }
+        const float2 s2 = team_moments<TEAM>(p.pre_kind, p.eps, inv, v, own);
+        if (p.stats != nullptr && active && t == 0) {
+            reinterpret_cast<float4*>(p.stats)[row] = make_float4(s1.x, s1.y, s2.x, s2.y);
+        }
+        if (p.n == nullptr || !active) continue;
+        const float2 r2 = both(s2.y), shift2 = both(-s2.x * s2.y);
+#pragma unroll
+        for (int k = 0; k < PACKS; ++k) {
+            if (!own.has(k)) continue;
+#pragma unroll
+            for (int e = 0; e < M; ++e) v[k][e] = fma2(v[k][e], r2, shift2);
+            if (p.pre_gamma != nullptr) {
+                own.fetch(p.pre_gamma, k, w);
+#pragma unroll
+                for (int e = 0; e < M; ++e) v[k][e] = mul2(v[k][e], w[e]);
+            }
+            if (p.pre_beta != nullptr) {
+                own.fetch(p.pre_beta, k, w);
+#pragma unroll
+                for (int e = 0; e < M; ++e) v[k][e] = add2(v[k][e], w[e]);
+            }
+            own.store(static_cast<T*>(p.n) + base, k, v[k]);
+        }
+    }
+}
+
+// Sums over rows: the teams of a CTA meet in shared memory, so that a CTA leaves one partial row.
+template <class T, int PACKS, bool VEC, int TEAM>
+__global__ void __launch_bounds__(kTeamThreads, 2)
+norm_residual_backward_team_kernel(const NormParams p) {
+    constexpr int N = Columns<T, VEC>::N, M = N / 2;
+    __shared__ float meet[kTeamThreads * 8];  // [teams][TEAM * 8]
+    const int t = threadIdx.x % TEAM;
+    const Columns<T, VEC> own{t, TEAM, 0, VEC ? p.cols / kPack<T> : p.cols};
+    const float inv = 1.0f / static_cast<float>(p.cols);
+    const bool gate_each = p.gate != nullptr && p.rows_per_gate == 1, gate_shared = p.gate != nullptr && !gate_each;
+    pdl_wait();
+    float2 acc[4][PACKS][M];
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+#pragma unroll
+        for (int k = 0; k < PACKS; ++k) {
+#pragma unroll
+            for (int e = 0; e < M; ++e) acc[a][k][e] = both(0.0f);
+        }
+    }
+    const int64_t teams = static_cast<int64_t>(gridDim.x) * (kTeamThreads / TEAM);
+    int64_t task = static_cast<int64_t>(blockIdx.x) * (kTeamThreads / TEAM) + threadIdx.x / TEAM;
+    const int64_t groups_rows = p.rows_per_gate == 1 ? p.rows : p.rows_per_gate;
+    for (int64_t first = task - threadIdx.x % kWarp / TEAM; first < p.tasks; first += teams, task += teams) {
+        const bool has_task = task < p.tasks;
+        const int64_t one = has_task ? task : p.tasks - 1;
+        const int64_t group = p.rows_per_gate == 1 ? 0 : one / p.tasks_per_gate;
+        const int64_t from = group * groups_rows + (one - group * p.tasks_per_gate) * p.rows_per_task;
+        const int64_t end = (group + 1) * groups_rows;
+        float2 gate[PACKS][M], gsum[PACKS][M];
+#pragma unroll
+        for (int k = 0; k < PACKS; ++k) {
+#pragma unroll
+            for (int e = 0; e < M; ++e) {
+                gate[k][e] = both(1.0f);
+                gsum[k][e] = both(0.0f);
+            }
+            if (gate_shared) {
+                own.stream(static_cast<const T*>(p.gate) + group * p.cols, k, gate[k]);
+                gate_pairs(p.gate_act, gate[k]);
+            }
+        }
+        for (int64_t i = 0; i < p.rows_per_task; ++i) {
+            const bool active = has_task && from + i < end;
+            const int64_t row = active ? from + i : 0, base = row * p.cols;
+            const float4 st = reinterpret_cast<const float4*>(p.stats_in)[row];
+            float2 d[PACKS][M], hat[PACKS][M], dy[PACKS][M], h[PACKS][M], w[M];
+#pragma unroll
+            for (int k = 0; k < PACKS; ++k) {
+#pragma unroll
+                for (int e = 0; e < M; ++e) d[k][e] = hat[k][e] = dy[k][e] = both(0.0f);
+                if (p.dn != nullptr) {
+                    own.stream(static_cast<const T*>(p.dn) + base, k, d[k]);
+                    own.stream(static_cast<const T*>(p.y_in) + base, k, hat[k]);
+                }
+                if (p.dy != nullptr) own.stream(static_cast<const T*>(p.dy) + base, k, dy[k]);
+                own.stream(static_cast<const T*>(p.h) + base, k, h[k]);
+                if (gate_each) {
+                    own.stream(static_cast<const T*>(p.gate) + base, k, gate[k]);
+                    gate_pairs(p.gate_act, gate[k]);
+                }
+            }
+            float level = 0.0f, along = 0.0f;
+            if (p.dn != nullptr) {
+                float2 sd = both(0.0f), sh = both(0.0f);
+                const float2 r = both(st.w), shift = both(-st.z * st.w);
+#pragma unroll
+                for (int k = 0; k < PACKS; ++k) {
+                    if (!own.has(k)) continue;
+                    if (p.pre_gamma != nullptr) own.fetch(p.pre_gamma, k, w);
+#pragma unroll
+                    for (int e = 0; e < M; ++e) {
+                        hat[k][e] = fma2(hat[k][e], r, shift);
+                        if (active) {
+                            acc[2][k][e] = fma2(d[k][e], hat[k][e], acc[2][k][e]);
+                            acc[3][k][e] = add2(acc[3][k][e], d[k][e]);
+                        }
+                        if (p.pre_gamma != nullptr) d[k][e] = mul2(d[k][e], w[e]);
+                        sd = add2(sd, d[k][e]);
+                        sh = fma2(d[k][e], hat[k][e], sh);
+                    }
+                }
+                if (p.pre_kind == FDL_NORM_LAYER) level = team_sum<TEAM>(sd.x + sd.y) * inv;
+                along = team_sum<TEAM>(sh.x + sh.y) * inv;
+            }
+            float2 sd = both(0.0f), sh = both(0.0f);
+            const float2 r2 = both(st.w), r1 = both(st.y), shift = both(-st.x * st.y);
+#pragma unroll
+            for (int k = 0; k < PACKS; ++k) {
+                if (!own.has(k)) continue;
+#pragma unroll
+                for (int e = 0; e < M; ++e) {
+                    d[k][e] = fma2(r2, fma2(hat[k][e], both(-along), add2(d[k][e], both(-level))), dy[k][e]);
+                    dy[k][e] = mul2(d[k][e], both(p.residual_scale));
+                    d[k][e] = mul2(d[k][e], both(p.block_scale));
+                    hat[k][e] = fma2(h[k][e], r1, shift);
+                    if (!own.inside(2 * e)) d[k][e].x = 0.0f;
+                    if (!own.inside(2 * e + 1)) d[k][e].y = 0.0f;
+                }
+                if (p.dx != nullptr && active) own.store(static_cast<T*>(p.dx) + base, k, dy[k]);
+                if (p.dgate != nullptr) {
+                    float2 u[M];
+                    own.fetch(p.post_gamma, k, u);
+#pragma unroll
+                    for (int e = 0; e < M; ++e) u[e] = mul2(u[e], hat[k][e]);
+                    if (p.post_beta != nullptr) {
+                        own.fetch(p.post_beta, k, w);
+#pragma unroll
+                        for (int e = 0; e < M; ++e) u[e] = add2(u[e], w[e]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < M; ++e) {
+                        u[e] = mul2(u[e], d[k][e]);
+                        if (active) gsum[k][e] = add2(gsum[k][e], u[e]);
+                    }
+                    if (gate_each && active) {
+                        times_slope_pairs(p.gate_act, gate[k], u);
+                        own.store(static_cast<T*>(p.dgate) + base, k, u);
+                    }
+                }
+                if (p.post_gamma != nullptr) own.fetch(p.post_gamma, k, w);
+#pragma unroll
+                for (int e = 0; e < M; ++e) {
+                    d[k][e] = mul2(d[k][e], gate[k][e]);
+                    if (active) {
+                        acc[0][k][e] = fma2(d[k][e], hat[k][e], acc[0][k][e]);
+                        acc[1][k][e] = add2(acc[1][k][e], d[k][e]);
+                    }
+                    if (p.post_gamma != nullptr) d[k][e] = mul2(d[k][e], w[e]);
+                    sd = add2(sd, d[k][e]);
+                    sh = fma2(d[k][e], hat[k][e], sh);
+                }
+            }
+            level = p.post_kind == FDL_NORM_LAYER ? team_sum<TEAM>(sd.x + sd.y) * inv : 0.0f;
+            along = p.post_kind != FDL_NORM_NONE ? team_sum<TEAM>(sh.x + sh.y) * inv : 0.0f;
+            if (p.dh == nullptr || !active) continue;
+#pragma unroll
+            for (int k = 0; k < PACKS; ++k) {
+                if (!own.has(k)) continue;
+#pragma unroll
+                for (int e = 0; e < M; ++e) d[k][e] = mul2(r1, fma2(hat[k][e], both(-along), add2(d[k][e], both(-level))));
+                own.store(static_cast<T*>(p.dh) + base, k, d[k]);
+            }
+        }
+        if (p.dgate == nullptr || !gate_shared || !has_task) continue;
+#pragma unroll
+        for (int k = 0; k < PACKS; ++k) {
+            if (!own.has(k)) continue;
+            times_slope_pairs(p.gate_act, gate[k], gsum[k]);
+            if (p.gate_partial == nullptr) {
+                own.store(static_cast<T*>(p.dgate) + group * p.cols, k, gsum[k]);
+                continue;
+            }
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                if (own.inside(e)) p.gate_partial[task * p.cols + own.col(k, e)] = e % 2 == 0 ? gsum[k][e / 2].x : gsum[k][e / 2].y;
+            }
+        }
+    }
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+        if (p.partial[a] == nullptr) continue;
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < PACKS; ++k) {
+            if (!own.has(k)) continue;
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                if (own.inside(e)) meet[threadIdx.x / TEAM * (TEAM * 8) + own.col(k, e)] = e % 2 == 0 ? acc[a][k][e / 2].x : acc[a][k][e / 2].y;
+            }
+        }
+        __syncthreads();
+        if (static_cast<int>(threadIdx.x) < p.cols) {
+            float s = meet[threadIdx.x];
+            for (int g = 1; g < kTeamThreads / TEAM; ++g) s += meet[g * (TEAM * 8) + threadIdx.x];
+            p.partial[a][static_cast<int64_t>(blockIdx.x) * p.cols + threadIdx.x] = s;
+        }
+    }
+}
 
 template <class T, int PACKS, bool VEC>
 __global__ void __launch_bounds__(512, 2)
@@ -1264,22 +1547,23 @@ norm_fold_kernel(const FoldJobs jobs) {
 // ---- launch shapes -------------------------------------------------------------------------------
 
 constexpr int kPerThread = 8;  // columns a thread owns
-constexpr int kWarpCols = kWarp * kPerThread;
+constexpr int kTeamCols = kWarp * kPerThread;
 constexpr int kMaxCols = kMaxCluster * 512 * kPerThread;
 
 struct Shape {
-    bool warp;     // a warp a row
+    int team;      // lanes of a row's team; 0: CTAs
     int threads;   // of a CTA
     int cluster;   // CTAs a row
     int blocks;    // CTAs that an SM is given
+    int rows() const { return team != 0 ? threads / team : 1; }  // of a CTA (or cluster) at a time
 };
 
-Shape shape_of(int64_t cols) {
-    if (cols <= kWarpCols) return {true, 256, 1, 4};
+Shape shape_of(int64_t cols, bool backward) {
+    if (cols <= kTeamCols) return {cols <= 8 * kPerThread ? 8 : cols <= 16 * kPerThread ? 16 : 32, kTeamThreads, 1, backward ? 2 : 4};
     int cluster = 1;
     while (cols > static_cast<int64_t>(cluster) * 512 * kPerThread) cluster *= 2;
     const int threads = static_cast<int>(ceil_div(ceil_div(cols, static_cast<int64_t>(cluster) * kPerThread), kWarp)) * kWarp;
-    return {false, threads, cluster, 1024 / threads < 1 ? 1 : 1024 / threads};
+    return {0, threads, cluster, 1024 / threads < 1 ? 1 : 1024 / threads};
 }
 
 // The ring form: columns of a CTA, its threads and its stages; stages == 0: does not fit.
@@ -1297,7 +1581,7 @@ struct RingShape {
 RingShape ring_shape(int64_t cols, int dtype, int tiles, int weights, bool backward, bool beta) {
     RingShape r = {};
     const int size = static_cast<int>(dtype_bytes(dtype)), n = 16 / size;
-    if (cols <= kWarpCols) return r;  // a warp a row
+    if (cols <= kTeamCols) return r;  // a team of lanes a row
     r.vec = cols % n == 0;
     r.per_thread = r.vec && dtype != FDL_F32 && !beta ? 16 : 8;
     r.cluster = 1;
@@ -1335,19 +1619,19 @@ struct BackwardPlan {
     Shape shape;      // direct form
     RingShape rshape; // ring form
     int64_t grid;     // CTAs
-    int64_t teams;    // partial rows of the sums over rows
+    int64_t partials; // partial rows of the sums over rows: one a CTA (or cluster)
     int64_t rows_per_gate, tasks_per_gate, rows_per_task, tasks;
 };
 
 // Tasks: every team gets about the same number of rows, and no task crosses a gate row's rows.
 BackwardPlan backward_plan(int64_t rows, int64_t cols, int64_t gate_rows, int sm_count, const RingShape* ring) {
     BackwardPlan b = {};
-    b.shape = shape_of(cols);
+    b.shape = shape_of(cols, true);
     b.ring = ring != nullptr;
     if (ring != nullptr) b.rshape = *ring;
     const int cluster = b.ring ? b.rshape.cluster : b.shape.cluster;
-    const int64_t per_cta = !b.ring && b.shape.warp ? b.shape.threads / kWarp : 1;
-    const int64_t slots = static_cast<int64_t>(sm_count) * (b.ring ? b.rshape.blocks : b.shape.blocks) / cluster;  // teams of CTAs
+    const int64_t per_cta = b.ring ? 1 : b.shape.rows();
+    const int64_t slots = static_cast<int64_t>(sm_count) * (b.ring ? b.rshape.blocks : b.shape.blocks) / cluster;  // (clusters of) CTAs
     const int64_t most = (slots < 1 ? 1 : slots) * per_cta;                                                        // teams at once
     const bool gate_each = gate_rows == rows;
     const int64_t groups = gate_rows == 0 || gate_each ? 1 : gate_rows;
@@ -1369,9 +1653,8 @@ BackwardPlan backward_plan(int64_t rows, int64_t cols, int64_t gate_rows, int sm
     b.rows_per_task = ceil_div(group, best);
     b.tasks_per_gate = ceil_div(group, b.rows_per_task);
     b.tasks = b.tasks_per_gate * groups;
-    b.teams = b.tasks < most ? b.tasks : most;
-    b.grid = ceil_div(b.teams, per_cta) * cluster;
-    b.teams = b.grid / cluster * per_cta;
+    b.partials = ceil_div(b.tasks < most ? b.tasks : most, per_cta);
+    b.grid = b.partials * cluster;
     return b;
 }
 
@@ -1396,33 +1679,28 @@ bool packs_fit(int dtype, int64_t cols, std::initializer_list<const void*> tenso
     return true;
 }
 
-template <template <class, int, int, bool> class Launch, class... Args>
-int dispatch(int dtype, bool vec, bool warp, Args&&... args) {
+int launch_direct(bool backward, int dtype, bool vec, const NormParams& p, const Shape& s, int64_t grid, cudaStream_t stream) {
     return with_dtype(dtype, [&](auto* tag) {
         using T = std::remove_pointer_t<decltype(tag)>;
         constexpr int N = kPack<T>;
-        if (vec) {
-            return warp ? Launch<T, N, kPerThread / N, true>::run(args...) : Launch<T, N, kPerThread / N, false>::run(args...);
+        auto launch = [&](auto forward_kernel, auto backward_kernel) {
+            return launch_ex(backward ? backward_kernel : forward_kernel, dim3(static_cast<unsigned int>(grid)), dim3(s.threads), 0, stream,
+                             dim3(s.cluster, 1, 1), tuning().pdl != 0, p);
+        };
+        if (s.team == 0) {
+            return vec ? launch(norm_residual_kernel<T, N, kPerThread / N>, norm_residual_backward_kernel<T, N, kPerThread / N>)
+                       : launch(norm_residual_kernel<T, 1, kPerThread>, norm_residual_backward_kernel<T, 1, kPerThread>);
         }
-        return warp ? Launch<T, 1, kPerThread, true>::run(args...) : Launch<T, 1, kPerThread, false>::run(args...);
+        auto team = [&](auto lanes) {
+            constexpr int L = decltype(lanes)::value;
+            return vec ? launch(norm_residual_team_kernel<T, kPerThread / N, true, L>, norm_residual_backward_team_kernel<T, kPerThread / N, true, L>)
+                       : launch(norm_residual_team_kernel<T, 1, false, L>, norm_residual_backward_team_kernel<T, 1, false, L>);
+        };
+        if (s.team == 8) return team(std::integral_constant<int, 8>{});
+        if (s.team == 16) return team(std::integral_constant<int, 16>{});
+        return team(std::integral_constant<int, 32>{});
     });
 }
-
-template <class T, int N, int PACKS, bool WARP>
-struct LaunchForward {
-    static int run(const NormParams& p, const Shape& s, int64_t grid, cudaStream_t stream) {
-        return launch_ex(norm_residual_kernel<T, N, PACKS, WARP>, dim3(static_cast<unsigned int>(grid)), dim3(s.threads), 0,
-                         stream, dim3(s.cluster, 1, 1), tuning().pdl != 0, p);
-    }
-};
-
-template <class T, int N, int PACKS, bool WARP>
-struct LaunchBackward {
-    static int run(const NormParams& p, const Shape& s, int64_t grid, cudaStream_t stream) {
-        return launch_ex(norm_residual_backward_kernel<T, N, PACKS, WARP>, dim3(static_cast<unsigned int>(grid)),
-                         dim3(s.threads), 0, stream, dim3(s.cluster, 1, 1), tuning().pdl != 0, p);
-    }
-};
 
 template <class K, class... Args>
 int launch_ring(K kernel, const NormParams& p, const RingShape& r, int64_t grid, cudaStream_t stream) {
@@ -1498,8 +1776,8 @@ int fdl_norm_residual(const void* x, const void* h, const void* gate, int64_t ga
     p.cols = static_cast<int>(cols);
     p.post_kind = post_kind; p.pre_kind = pre_kind; p.gate_act = gate_act;
     p.residual_scale = residual_scale; p.block_scale = block_scale; p.eps = eps;
-    const bool vec = packs_fit(dtype, cols, {x, h, gate, y, n});
-    const Shape s = shape_of(cols);
+    const bool vec = packs_fit(dtype, cols, {x, h, gate, y, n, post_gamma, post_beta, pre_gamma, pre_beta});
+    const Shape s = shape_of(cols, false);
     const RingShape r = ring_shape(cols, dtype, 2 + (gate != nullptr && gate_rows == rows), 0, false, false);
     if (ring_fits(r, {x, h, gate}, {y, n, post_gamma, post_beta, pre_gamma, pre_beta})) {
         const int64_t teams = static_cast<int64_t>(info->sm_count) * r.blocks / r.cluster;
@@ -1509,11 +1787,10 @@ int fdl_norm_residual(const void* x, const void* h, const void* gate, int64_t ga
             return launch_ring_forward(dtype, p, r, teams * r.cluster, as_stream(stream));
         }
     }
-    const int64_t per_cta = s.warp ? s.threads / kWarp : 1;
     const int64_t slots = static_cast<int64_t>(info->sm_count) * s.blocks / s.cluster;
-    const int64_t work = ceil_div(rows, per_cta);
+    const int64_t work = ceil_div(rows, static_cast<int64_t>(s.rows()));
     const int64_t grid = (work < slots ? work : slots < 1 ? 1 : slots) * s.cluster;
-    return dispatch<LaunchForward>(dtype, vec, s.warp, p, s, grid, as_stream(stream));
+    return launch_direct(false, dtype, vec, p, s, grid, as_stream(stream));
 }
 
 // Room for whichever form the call takes: the direct form, or the ring form with any of its tiles and types.
@@ -1527,7 +1804,7 @@ size_t fdl_norm_residual_backward_scratch_bytes(int64_t rows, int64_t cols, int6
     auto add = [&](const RingShape* r) {
         const BackwardPlan b = backward_plan(rows, cols, gate_rows, sms, r);
         const int64_t gate_part = gate_rows == 0 || gate_rows == rows || b.tasks_per_gate == 1 ? 0 : b.tasks;
-        const int64_t f = (4 * b.teams + gate_part) * cols;
+        const int64_t f = (4 * b.partials + gate_part) * cols;
         if (f > floats) floats = f;
     };
     add(nullptr);
@@ -1580,7 +1857,7 @@ int fdl_norm_residual_backward(const void* dy, const void* dn, const void* y, co
     }
     const DeviceInfo* info = current_device_info(&status);
     if (info == nullptr) return status;
-    const bool vec = packs_fit(dtype, cols, {dy, dn, y, h, gate, dx, dh, dgate});
+    const bool vec = packs_fit(dtype, cols, {dy, dn, y, h, gate, dx, dh, dgate, post_gamma, post_beta, pre_gamma});
     const bool beta = dpost_beta != nullptr || dpre_beta != nullptr || (post_beta != nullptr && dgate != nullptr);
     const int tiles = 1 + (dn != nullptr ? 2 : 0) + (dy != nullptr) + (gate != nullptr && gate_rows == rows);
     const RingShape r = ring_shape(cols, dtype, tiles, 2, true, beta);
@@ -1606,8 +1883,8 @@ int fdl_norm_residual_backward(const void* dy, const void* dn, const void* y, co
     for (int a = 0; a < 4; ++a) {
         if (sums[a] == nullptr) continue;
         p.partial[a] = at;
-        jobs.job[njobs++] = {at, sums[a], FDL_F32, 1, b.teams};
-        at += b.teams * cols;
+        jobs.job[njobs++] = {at, sums[a], FDL_F32, 1, b.partials};
+        at += b.partials * cols;
     }
     if (dgate != nullptr && gate_rows != rows && b.tasks_per_gate > 1) {
         p.gate_partial = at;
@@ -1618,12 +1895,12 @@ int fdl_norm_residual_backward(const void* dy, const void* dn, const void* y, co
         status = error_flag_device_ptr(&p.error_flag);
         if (status == FDL_OK) status = launch_ring_backward(dtype, beta, p, r, b.grid, s);
     } else {
-        status = dispatch<LaunchBackward>(dtype, vec, b.shape.warp, p, b.shape, b.grid, s);
+        status = launch_direct(true, dtype, vec, p, b.shape, b.grid, s);
     }
     if (status != FDL_OK || njobs == 0) return status;
     const dim3 grid(static_cast<unsigned int>(ceil_div(cols, kFoldX)), static_cast<unsigned int>(njobs),
                     static_cast<unsigned int>(groups < 64 ? groups : 64));
-    const int strands = b.teams <= 64 ? 4 : b.teams <= 256 ? 8 : b.teams <= 512 ? 16 : kFoldY;
+    const int strands = b.partials <= 64 ? 4 : b.partials <= 256 ? 8 : b.partials <= 512 ? 16 : kFoldY;
     return launch_ex(norm_fold_kernel, grid, dim3(kFoldX, strands), 0, s, dim3(1, 1, 1), tuning().pdl != 0, jobs);
 }
 
