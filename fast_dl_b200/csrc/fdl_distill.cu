@@ -6,7 +6,7 @@
 //   log q_v = (z_v - m) / T - log S,             m = max z, S = sum_v exp((z_v - m) / T),
 //   row_loss = sum_j p_j (log p_j - log q_{i_j}),    loss = scale * sum_r w_r row_loss_r,
 //   dz_v = scale w_r / T * (P q_v - sum of the p_j whose i_j is v),    P = sum_j p_j.
-// A row of weight 0 or without entries that count is left out: loss 0, gradient 0, its logits not read.
+// A row of weight 0 or without entries that count is left out: loss 0, gradient 0, whatever its logits hold.
 //
 // Differences of logarithms are taken in 64 bits (k of them a row): where teacher and student
 // agree, the loss is a small difference of numbers of size ten.
@@ -51,30 +51,6 @@ __device__ __forceinline__ float load_any(const void* p, int dtype, int64_t i) {
 // exp((a - b) / T) for a running maximum a <= b, with c = log2(e) / T; 1 when both are -inf.
 __device__ __forceinline__ float exp_diff(float a, float b, float c) { return a == b ? 1.0f : ex2_approx((a - b) * c); }
 
-template <int kWarps>
-__device__ __forceinline__ float block_max(float v, float* red) {
-    v = warp_max(v);
-    __syncthreads();
-    if ((threadIdx.x & (kWarp - 1)) == 0) red[threadIdx.x / kWarp] = v;
-    __syncthreads();
-    v = red[0];
-#pragma unroll
-    for (int w = 1; w < kWarps; ++w) v = fmaxf(v, red[w]);
-    return v;
-}
-
-template <int kWarps, class S>
-__device__ __forceinline__ S block_sum(S v, S* red) {
-    v = warp_sum(v);
-    __syncthreads();
-    if ((threadIdx.x & (kWarp - 1)) == 0) red[threadIdx.x / kWarp] = v;
-    __syncthreads();
-    v = red[0];
-#pragma unroll
-    for (int w = 1; w < kWarps; ++w) v += red[w];
-    return v;
-}
-
 // A row as a head and a tail of single elements around aligned 128-bit packs.
 template <class T>
 struct RowSpan {
@@ -87,149 +63,317 @@ struct RowSpan {
     }
 };
 
-// Short rows: a small CTA a row, many of them an SM, the row read a second time (out of L1 or L2) for its gradient.
-constexpr int kRowThreads = 128;
+// What the teacher says of a row, in the shared memory of the warp that read it.
+struct Entries {
+    float* prob;  // [k]: p_j; of entries that share a column the first has the sum
+    float* here;  // [k]: the student's logit there
+    int* at;      // [k]: the column, or -1: does not count, or folded into another
+    uint16_t* table;
+    int places;   // of the table, a power of two of at least 2 k
+};
 
-template <class T, bool LOSS, bool GRAD>
-__global__ void __launch_bounds__(kRowThreads)
-distill_rows_kernel(const DistillParams p) {
-    constexpr int N = kPack<T>, kThreads = kRowThreads, kWarps = kThreads / kWarp;
-    __shared__ float prob[kMaxEntries];
-    __shared__ int at[kMaxEntries];
-    __shared__ float here[kMaxEntries];
-    __shared__ float redf[kWarps];
-    __shared__ double redd[kWarps];
-    const int t = threadIdx.x;
-    const float c = static_cast<float>(kLog2e * p.inv_temperature);
-    pdl_wait();
-    for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-        const T* z = static_cast<const T*>(p.logits) + row * p.logits_stride;
-        const float weight = p.row_weight == nullptr ? 1.0f : p.row_weight[row];
-        // The teacher's entries.
-        float top = -INFINITY;
-        for (int j = t; j < p.k; j += kThreads) {
-            const int64_t i = p.index[row * p.k + j];
-            const bool valid = i >= 0 && i < p.vocab;
-            const float v = valid ? load_any(p.teacher, p.teacher_dtype, row * p.k + j) : -INFINITY;
-            prob[j] = v;
-            at[j] = v > -INFINITY ? static_cast<int>(i) : -1;  // a NaN does not count either
-            top = fmaxf(top, v);
-        }
-        top = block_max<kWarps>(top, redf);
-        const bool live = weight != 0.0f && top != -INFINITY;
-        T* g = GRAD ? static_cast<T*>(p.grad) + row * p.grad_stride : nullptr;
-        if (!live) {
-            if (LOSS && t == 0) {
-                p.row_loss[row] = 0.0f;
-                p.row_stats[2 * row] = 0.0f;
-                p.row_stats[2 * row + 1] = 0.0f;
-            }
-            if (GRAD) {
-                for (int i = t; i < p.vocab; i += kThreads) g[i] = from_f32<T>(0.0f);
-            }
-            __syncthreads();
-            continue;
-        }
-        float part = 0.0f;
-        for (int j = t; j < p.k; j += kThreads) {
-            if (at[j] >= 0) {
-                here[j] = to_f32(z[at[j]]);
-                part += ex2_approx((prob[j] - top) * c);
-            }
-        }
-        const float teacher_sum = block_sum<kWarps>(part, redf);
-        const double log_norm = p.teacher_lse == nullptr
-                                    ? static_cast<double>(top) * p.inv_temperature + log(static_cast<double>(teacher_sum))
-                                    : static_cast<double>(p.teacher_lse[row]);
-        // The student's statistics.
-        float m, total;
-        if (LOSS) {
-            const RowSpan<T> span(z, p.vocab);
-            const T* body = z + span.head;
-            float mx = -INFINITY, s = 0.0f;
-            for (int i = t; i < span.packs; i += kThreads) {
-                float v[N];
-                Chunk<T, N>::load(body + static_cast<int64_t>(i) * N, v);
-                float big = v[0];
+// One warp reads a row's entries.  Returns whether any counts, and then the loss's share that does not need the
+// row's sum, base = sum p_j (log p_j - logit_j / T), and mass = sum p_j.  `wanted`: columns whose logits to read.
+template <class T, bool LOSS, bool GRAD, class Wanted>
+__device__ __forceinline__ bool read_entries(const DistillParams& p, const T* z, int64_t row, float c, const Entries& out, double* base_out,
+                                             double* mass_out, Wanted&& wanted) {
+    const int lane = threadIdx.x & (kWarp - 1);
+    float* const prob = out.prob;
+    float* const here = out.here;
+    int* const at = out.at;
+    float top = -INFINITY;
+    for (int j0 = lane; j0 < p.k; j0 += 4 * kWarp) {  // four entries' loads at a time
+        int64_t i[4];
+        float v[4];
 #pragma unroll
-                for (int e = 1; e < N; ++e) big = fmaxf(big, v[e]);
-                const float now = fmaxf(mx, big);
-                const float ref = now == -INFINITY ? 0.0f : now;  // nothing but -inf so far: exp(-inf) each
-                float add = 0.0f;
-#pragma unroll
-                for (int e = 0; e < N; ++e) add += ex2_approx((v[e] - ref) * c);
-                s = s * exp_diff(mx, now, c) + add;
-                mx = now;
-            }
-            if (t < span.head + span.tail) {
-                const float v = to_f32(t < span.head ? z[t] : z[p.vocab - 1 - (t - span.head)]);
-                const float now = fmaxf(mx, v);
-                s = s * exp_diff(mx, now, c) + ex2_approx((v - (now == -INFINITY ? 0.0f : now)) * c);
-                mx = now;
-            }
-            m = block_max<kWarps>(mx, redf);
-            total = block_sum<kWarps>(s * exp_diff(mx, m, c), redf);
-            if (t == 0) {
-                p.row_stats[2 * row] = m;
-                p.row_stats[2 * row + 1] = total;
-            }
-        } else {
-            m = p.row_stats[2 * row];
-            total = p.row_stats[2 * row + 1];
+        for (int q = 0; q < 4; ++q) {
+            const int64_t from = row * p.k + min(j0 + q * kWarp, p.k - 1);
+            i[q] = p.index[from];
+            v[q] = load_any(p.teacher, p.teacher_dtype, from);
         }
-        const double log_total = log(static_cast<double>(total));
-        double kl = 0.0;
-        float mass = 0.0f;
-        for (int j = t; j < p.k; j += kThreads) {
-            float pj = 0.0f;
-            if (at[j] >= 0) {
-                const double logp = static_cast<double>(prob[j]) * p.inv_temperature - log_norm;
-                pj = expf(static_cast<float>(logp));
-                const double logq = (static_cast<double>(here[j]) - m) * p.inv_temperature - log_total;
-                if (pj != 0.0f) kl += pj * (logp - logq);
-            }
-            prob[j] = pj;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int j = j0 + q * kWarp;
+            if (j >= p.k) break;
+            const bool counts = i[q] >= 0 && i[q] < p.vocab && v[q] > -INFINITY;  // a NaN does not either
+            prob[j] = counts ? v[q] : -INFINITY;
+            at[j] = counts ? static_cast<int>(i[q]) : -1;
+            if (counts) top = fmaxf(top, v[q]);
+        }
+    }
+    top = warp_max(top);
+    if (top == -INFINITY) return false;
+    float part = 0.0f;
+    for (int j0 = lane; j0 < p.k; j0 += 4 * kWarp) {
+        float v[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int j = j0 + q * kWarp;
+            const int col = j < p.k ? at[j] : -1;
+            v[q] = col >= 0 && wanted(col) ? to_f32(z[col]) : 0.0f;
+            if (col >= 0) part += ex2_approx((prob[j] - top) * c);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            if (j0 + q * kWarp < p.k) here[j0 + q * kWarp] = v[q];
+        }
+    }
+    const double sum = static_cast<double>(warp_sum(part));
+    const double norm = p.teacher_lse == nullptr ? static_cast<double>(top) * p.inv_temperature + log(sum)
+                                                 : static_cast<double>(p.teacher_lse[row]);
+    double base = 0.0, mass = 0.0;
+    for (int j = lane; j < p.k; j += kWarp) {
+        float pj = 0.0f;
+        if (at[j] >= 0) {
+            const double logp = static_cast<double>(prob[j]) * p.inv_temperature - norm;
+            pj = expf(static_cast<float>(logp));
+            if (LOSS && pj != 0.0f) base += pj * (logp - static_cast<double>(here[j]) * p.inv_temperature);
             mass += pj;
         }
-        if (LOSS) {
-            kl = block_sum<kWarps>(kl, redd);
-            if (t == 0) p.row_loss[row] = static_cast<float>(kl);
+        prob[j] = pj;
+    }
+    *base_out = warp_sum(base);
+    *mass_out = warp_sum(mass);
+    if (!GRAD) return true;
+    // Entries of one column: each entry writes its number into the column's place of a hash table
+    // and looks who is there.  Another column there: again with another hash (that column's own
+    // entries are all in the same position); its own column: to be folded.  What the table held
+    // before does not matter, as a place is read after at least one entry wrote it.
+    uint32_t pending = 0, same = 0;  // bit q: entry lane + 32 q
+    for (int j = lane, q = 0; j < p.k; j += kWarp, ++q) pending |= at[j] >= 0 ? 1u << q : 0u;
+    for (uint32_t round = 0; __any_sync(kFullMask, pending != 0u); ++round) {
+        const uint32_t mix = 0x9E3779B1u + 2u * round * 0x85EBCA6Bu;  // odd
+        __syncwarp();
+        for (uint32_t left = pending; left != 0u; left &= left - 1u) {
+            const int j = lane + kWarp * (__ffs(left) - 1);
+            out.table[(static_cast<uint32_t>(at[j] + 1) * mix >> 15) & (out.places - 1)] = static_cast<uint16_t>(j);
         }
-        if (GRAD) {
-            mass = block_sum<kWarps>(mass, redf);
-            if (p.teacher_lse == nullptr) mass = mass == mass ? 1.0f : mass;
-            float coef = p.scale * weight * static_cast<float>(p.inv_temperature);
-            if (p.grad_loss != nullptr) coef *= *p.grad_loss;
-            const float each = coef * mass / total;
-            // In place: every read of the row (above) is done before the first write.
-            const RowSpan<T> span(z, p.vocab);
-            const bool same_phase = ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(g)) & 15) == 0;
-            const int head = same_phase ? span.head : 0, packs = same_phase ? span.packs : 0;
-            for (int i = t; i < packs; i += kThreads) {
-                float v[N];
-                Chunk<T, N>::load(z + head + static_cast<int64_t>(i) * N, v);
+        __syncwarp();
+        for (uint32_t left = pending; left != 0u; left &= left - 1u) {
+            const int q = __ffs(left) - 1, j = lane + kWarp * q;
+            const int w = out.table[(static_cast<uint32_t>(at[j] + 1) * mix >> 15) & (out.places - 1)];
+            if (w == j || at[w] == at[j]) {
+                pending &= ~(1u << q);
+                if (w != j) same |= 1u << q;
+            }
+        }
+    }
+    __syncwarp();
+    // The first entry of a shared column gets the sum (in entry order over lanes, a fixed tree); the
+    // others are dropped.
+    for (uint32_t owners = __ballot_sync(kFullMask, same != 0u); owners != 0u; owners = __ballot_sync(kFullMask, same != 0u)) {
+        const int owner = __ffs(owners) - 1;
+        const int j = __shfl_sync(kFullMask, same != 0u ? lane + kWarp * (__ffs(same) - 1) : 0, owner);
+        if (lane == owner) same &= same - 1u;
+        const int col = at[j];
+        if (col < 0) continue;  // dropped with an earlier one
+        int least = p.k;
+        float sum_p = 0.0f;
+        for (int i = lane; i < p.k; i += kWarp) {
+            if (at[i] == col) {
+                least = min(least, i);
+                sum_p += prob[i];
+            }
+        }
+        least = __reduce_min_sync(kFullMask, least);
+        sum_p = warp_sum(sum_p);
+        __syncwarp();
+        for (int i = lane; i < p.k; i += kWarp) {
+            if (at[i] == col) {
+                if (i == least) prob[i] = sum_p;
+                else at[i] = -1;
+            }
+        }
+        __syncwarp();
+    }
+    return true;
+}
+
+// -inf in each element of a pack.
+__device__ __forceinline__ uint4 lowest_pack(float) { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
+__device__ __forceinline__ uint4 lowest_pack(__half) { return make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u); }
+__device__ __forceinline__ uint4 lowest_pack(__nv_bfloat16) { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
+
+// A running maximum and sum of exponentials relative to it.
+struct Running {
+    float m = -INFINITY, s = 0.0f;
+    template <class T, int PACKS>
+    __device__ __forceinline__ void take(const uint4 (&raw)[PACKS], float c) {
+        constexpr int M = kPack<T> / 2;
+        float big = -INFINITY;
 #pragma unroll
-                for (int e = 0; e < N; ++e) v[e] = ex2_approx((v[e] - m) * c) * each;
-                Chunk<T, N>::store_stream(g + head + static_cast<int64_t>(i) * N, v);
-            }
-            for (int i = t; i < p.vocab - packs * N; i += kThreads) {
-                const int col = i < head ? i : i + packs * N;
-                g[col] = from_f32<T>(ex2_approx((to_f32(z[col]) - m) * c) * each);
-            }
-            __syncthreads();
-            // The teacher's places, written after the dense part (same CTA, behind a barrier).  An
-            // index that is there twice is written by its first entry, with the sum in entry order.
-            for (int j = t; j < p.k; j += kThreads) {
-                if (at[j] < 0) continue;
-                bool first = true;
-                for (int i = 0; i < j; ++i) first = first && at[i] != at[j];
-                if (!first) continue;
-                float sum = 0.0f;
-                for (int i = j; i < p.k; ++i) sum += at[i] == at[j] ? prob[i] : 0.0f;
-                g[at[j]] = from_f32<T>(coef * (mass * (ex2_approx((here[j] - m) * c) / total) - sum));
+        for (int q = 0; q < PACKS; ++q) {
+            float2 v[M];
+            unpack2(raw[q], v, T{});
+#pragma unroll
+            for (int e = 0; e < M; ++e) big = fmaxf(big, fmaxf(v[e].x, v[e].y));
+        }
+        const float now = fmaxf(m, big);
+        const float ref = now == -INFINITY ? 0.0f : now;  // nothing but -inf so far: exp(-inf) each
+        const float2 down = both(-ref), c2 = both(c);
+        float2 add[2] = {both(0.0f), both(0.0f)};
+#pragma unroll
+        for (int q = 0; q < PACKS; ++q) {
+            float2 v[M];
+            unpack2(raw[q], v, T{});
+#pragma unroll
+            for (int e = 0; e < M; ++e) {
+                v[e] = mul2(add2(v[e], down), c2);
+                add[e & 1] = add2(add[e & 1], make_float2(ex2_approx(v[e].x), ex2_approx(v[e].y)));
             }
         }
-        __syncthreads();
+        const float2 sum = add2(add[0], add[1]);
+        s = s * exp_diff(m, now, c) + (sum.x + sum.y);
+        m = now;
+    }
+    __device__ __forceinline__ void take_one(float v, float c) {
+        const float now = fmaxf(m, v);
+        s = s * exp_diff(m, now, c) + ex2_approx((v - (now == -INFINITY ? 0.0f : now)) * c);
+        m = now;
+    }
+    // The warp's pair, in every lane.
+    __device__ __forceinline__ float2 of_warp(float c) const {
+        const float top = warp_max(m);
+        return make_float2(top, warp_sum(s * exp_diff(m, top, c)));
+    }
+};
+
+// The row's maximum and sum from the warps' pairs: the same order, and so the same bits, in every warp and CTA.
+__device__ __forceinline__ float2 fold_stats(const float2* stat, int n, float c) {
+    const int lane = threadIdx.x & (kWarp - 1);
+    float m = -INFINITY;
+    for (int i = lane; i < n; i += kWarp) m = fmaxf(m, stat[i].x);
+    m = warp_max(m);
+    float sum = 0.0f;
+    for (int i = lane; i < n; i += kWarp) sum += stat[i].y * exp_diff(stat[i].x, m, c);
+    return make_float2(m, warp_sum(sum));
+}
+__device__ __forceinline__ void write_loss(const DistillParams& p, double base, double mass, int64_t row, float2 f) {
+    p.row_stats[2 * row] = f.x;
+    p.row_stats[2 * row + 1] = f.y;
+    p.row_loss[row] =
+        static_cast<float>(base + mass * (static_cast<double>(f.x) * p.inv_temperature + log(static_cast<double>(f.y))));
+}
+__device__ __forceinline__ void write_left_out(const DistillParams& p, int64_t row) {
+    p.row_stats[2 * row] = 0.0f;
+    p.row_stats[2 * row + 1] = 0.0f;
+    p.row_loss[row] = 0.0f;
+}
+
+// ---- short rows: in the registers of a warp or of a CTA -------------------------------------------------
+//
+// WARPS warps a row, up to HELD packs a thread: rows of up to 4 KiB a warp.  With one warp a row there is no barrier
+// at all; otherwise the first warp reads the entries while all of them have the row on its way, and one barrier
+// brings the warps' pairs and the entries together.  What bounds it is the chain of dependent loads (entries, the
+// logits that they name), so as many rows as the registers allow are under way at once, and the row is asked for
+// before it is known to count.
+
+constexpr int kHeld = 8;  // the most
+
+template <class T, bool LOSS, bool GRAD, int WARPS, int HELD>
+__global__ void __launch_bounds__(WARPS == 1 ? 256 : WARPS * kWarp, WARPS == 1 ? (HELD <= 4 ? 4 : 3) : 24 / WARPS)
+distill_rows_kernel(const DistillParams p, int places) {
+    constexpr int N = kPack<T>, M = N / 2;
+    constexpr int kTeams = WARPS == 1 ? 256 / kWarp : 1, kThreads = WARPS * kWarp;
+    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ float2 stat[WARPS];
+    __shared__ double shared_base, shared_mass;
+    __shared__ int shared_live;
+    const int lane = threadIdx.x & (kWarp - 1), warp = threadIdx.x / kWarp;
+    const int team = WARPS == 1 ? warp : 0, w = WARPS == 1 ? 0 : warp, t = w * kWarp + lane;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * kTeams + team;
+    if (row >= p.rows) return;
+    const float c = static_cast<float>(kLog2e * p.inv_temperature);
+    float* const probs = reinterpret_cast<float*>(smem) + team * 3 * p.k;
+    const Entries entries{probs, probs + p.k, reinterpret_cast<int*>(probs + 2 * p.k),
+                          reinterpret_cast<uint16_t*>(reinterpret_cast<float*>(smem) + kTeams * 3 * p.k) + team * places, places};
+    pdl_wait();
+    const T* z = static_cast<const T*>(p.logits) + row * p.logits_stride;
+    T* const g = GRAD ? static_cast<T*>(p.grad) + row * p.grad_stride : nullptr;
+    const RowSpan<T> span(z, p.vocab);
+    const bool same_phase = ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(g)) & 15) == 0;
+    const float weight = p.row_weight == nullptr ? 1.0f : p.row_weight[row];
+    uint4 raw[HELD];
+    float edge = -INFINITY;
+    const int edges = span.head + span.tail;
+    const int edge_col = lane < span.head ? lane : p.vocab - span.tail + (lane - span.head);
+    double base = 0.0, mass = 0.0;
+    const uint4* packs = reinterpret_cast<const uint4*>(z + span.head);
+#pragma unroll
+    for (int q = 0; q < HELD; ++q) raw[q] = t + q * kThreads < span.packs ? packs[t + q * kThreads] : lowest_pack(T{});
+    if (w == 0 && lane < edges) edge = to_f32(z[edge_col]);
+    bool live = weight != 0.0f;
+    if (live) {
+        if (w == 0) {
+            live = read_entries<T, LOSS, GRAD>(p, z, row, c, entries, &base, &mass, [](int) { return true; });
+            if (WARPS > 1 && lane == 0) {
+                shared_base = base;
+                shared_mass = mass;
+                shared_live = live;
+            }
+        }
+    }
+    float2 f = make_float2(0.0f, 1.0f);
+    if (weight != 0.0f) {
+        if (LOSS) {
+            Running run;
+            run.take<T>(raw, c);
+            if (w == 0 && lane < edges) run.take_one(edge, c);
+            f = run.of_warp(c);
+            if (WARPS > 1 && lane == 0) stat[w] = f;
+        }
+        if (WARPS > 1) {
+            __syncthreads();
+            live = shared_live != 0;
+            mass = shared_mass;
+            if (LOSS) f = fold_stats(stat, WARPS, c);
+        }
+    }
+    if (!live) {
+        if (LOSS && t == 0) write_left_out(p, row);
+        if (GRAD) {
+            for (int i = t; i < p.vocab; i += kThreads) g[i] = from_f32<T>(0.0f);
+        }
+        return;
+    }
+    if (LOSS && t == 0) write_loss(p, base, mass, row, f);
+    if (!LOSS) f = make_float2(p.row_stats[2 * row], p.row_stats[2 * row + 1]);
+    if (!GRAD) return;
+    const float coef = p.scale * static_cast<float>(p.inv_temperature) * (p.grad_loss != nullptr ? *p.grad_loss : 1.0f) * weight;
+    const float part = p.teacher_lse == nullptr && mass == mass ? 1.0f : static_cast<float>(mass);
+    const float each = coef * part / f.y;
+    const float2 down = both(-f.x), c2 = both(c), each2 = both(each);
+#pragma unroll
+    for (int q = 0; q < HELD; ++q) {
+        const int i = t + q * kThreads;
+        if (i >= span.packs) break;
+        float2 v[M];
+        unpack2(raw[q], v, T{});
+#pragma unroll
+        for (int e = 0; e < M; ++e) {
+            v[e] = mul2(add2(v[e], down), c2);
+            v[e] = mul2(make_float2(ex2_approx(v[e].x), ex2_approx(v[e].y)), each2);
+        }
+        T* const out = g + span.head + static_cast<int64_t>(i) * N;
+        if (same_phase) {
+            store_pairs(out, v);
+        } else {
+#pragma unroll
+            for (int e = 0; e < M; ++e) {
+                out[2 * e] = from_f32<T>(v[e].x);
+                out[2 * e + 1] = from_f32<T>(v[e].y);
+            }
+        }
+    }
+    if (w == 0 && lane < edges) g[edge_col] = from_f32<T>(ex2_approx((edge - f.x) * c) * each);
+    // The columns that the teacher names, behind the dense part.
+    if (WARPS > 1) __syncthreads();
+    else __syncwarp();
+    for (int j = t; j < p.k; j += kThreads) {
+        const int col = entries.at[j];
+        if (col < 0) continue;
+        const float q = ex2_approx((entries.here[j] - f.x) * c) / f.y;
+        g[col] = from_f32<T>(coef * (part * q - entries.prob[j]));
     }
 }
 
@@ -246,8 +390,10 @@ distill_rows_kernel(const DistillParams p) {
 //   writes   eight warps wait for the pairs, fold them, write the gradient chunk by chunk and give the places back.
 // So a row is read once and its gradient written once; the sums of row i + 1 are under way while the gradient of
 // row i is written, and the exchange between them falls to nobody's wait as long as the ring holds more than
-// the row.  The loss alone has two groups of eight warps for the sums, which take the chunks in turn, the
-// gradient alone two groups for the writes.
+// the row.  The loss alone has two groups of eight warps for the sums, one for the even and one for the odd places of
+// the ring, the gradient alone two groups for the writes.  (A barrier tells one round of its place from the next
+// only, so whoever waits for a place has to wait for each of its rounds: with the chunks of a row dealt out in
+// turn, a group could be two rounds ahead of a slow copy and take the place's last chunk for its next.)
 // The elements of a row outside its 16-byte grid (its first and last few) go by plain loads.
 //
 // Every wait has a limit; one that gives up ends all of them (and is reported through the error flag).
@@ -345,11 +491,6 @@ __device__ __forceinline__ bool stat_wait(int cluster, uint64_t* bar, uint32_t p
     return cluster == 1 ? warp_wait(bar, parity, failed, error_flag) : warp_wait<true>(bar, parity, failed, error_flag);
 }
 
-// -inf in each element of a pack.
-__device__ __forceinline__ uint4 lowest_pack(float) { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
-__device__ __forceinline__ uint4 lowest_pack(__half) { return make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u); }
-__device__ __forceinline__ uint4 lowest_pack(__nv_bfloat16) { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
-
 // A position in a ring of `size` places: place and the parity of its round.
 struct RingPlace {
     int place;
@@ -391,35 +532,13 @@ struct Slice {
     }
 };
 
-// The row's maximum and sum from the warps' pairs: the same order, and so the same bits, in every warp and CTA.
-__device__ __forceinline__ float2 fold_stats(const float2* stat, int n, float c) {
-    const int lane = threadIdx.x & (kWarp - 1);
-    float m = -INFINITY;
-    for (int i = lane; i < n; i += kWarp) m = fmaxf(m, stat[i].x);
-    m = warp_max(m);
-    float sum = 0.0f;
-    for (int i = lane; i < n; i += kWarp) sum += stat[i].y * exp_diff(stat[i].x, m, c);
-    return make_float2(m, warp_sum(sum));
-}
-__device__ __forceinline__ void write_loss(const DistillParams& p, const Prepared& pre, int64_t row, float2 f) {
-    p.row_stats[2 * row] = f.x;
-    p.row_stats[2 * row + 1] = f.y;
-    p.row_loss[row] = static_cast<float>(
-        pre.base + pre.mass * (static_cast<double>(f.x) * p.inv_temperature + log(static_cast<double>(f.y))));
-}
-__device__ __forceinline__ void write_left_out(const DistillParams& p, int64_t row) {
-    p.row_stats[2 * row] = 0.0f;
-    p.row_stats[2 * row + 1] = 0.0f;
-    p.row_loss[row] = 0.0f;
-}
-
 template <class T, bool LOSS, bool GRAD>
 __global__ void __launch_bounds__(kRingThreads, 1)
 distill_ring_kernel(const RingParams r) {
     constexpr int N = kPack<T>;
     constexpr int kSumGroups = !LOSS ? 0 : GRAD ? 1 : 2, kWriteGroups = !GRAD ? 0 : LOSS ? 1 : 2;
     constexpr int kSumWarps = kSumGroups * kGroupWarps;
-    extern __shared__ __align__(128) unsigned char smem[];
+    extern __shared__ __align__(16) unsigned char smem[];
     __shared__ uint64_t full[kMaxSlots], empty[kMaxSlots], prep_full[kPrepSlots], prep_empty[kPrepSlots], stat_full[kStatSlots];
     __shared__ float2 stat[LOSS ? kStatSlots : 1][kMaxCluster * (GRAD ? 1 : 2) * kGroupWarps];
     __shared__ Prepared prepared[kPrepSlots];
@@ -494,123 +613,17 @@ distill_ring_kernel(const RingParams r) {
             const int place = static_cast<int>(number % kPrepSlots);
             // The first round finds the slots free.
             if (!warp_wait(&prep_empty[place], static_cast<uint32_t>(number / kPrepSlots & 1) ^ 1u, failed, r.error_flag)) break;
-            float* const prob = probs + place * p.k;
-            float* const here = heres + place * p.k;
-            int* const at = ats + place * p.k;
             Prepared& out = prepared[place];
             const T* z = static_cast<const T*>(p.logits) + row * p.logits_stride;
+            const Slice<T> slice(z, p.vocab, rank, log2_cluster);
             const float weight = p.row_weight == nullptr ? 1.0f : p.row_weight[row];
-            float top = -INFINITY;
-            for (int j0 = lane; j0 < p.k; j0 += 4 * kWarp) {  // four entries' loads at a time
-                int64_t i[4];
-                float v[4];
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int64_t from = row * p.k + min(j0 + q * kWarp, p.k - 1);
-                    i[q] = p.index[from];
-                    v[q] = load_any(p.teacher, p.teacher_dtype, from);
-                }
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int j = j0 + q * kWarp;
-                    if (j >= p.k) break;
-                    const bool counts = i[q] >= 0 && i[q] < p.vocab && v[q] > -INFINITY;  // a NaN does not either
-                    prob[j] = counts ? v[q] : -INFINITY;
-                    at[j] = counts ? static_cast<int>(i[q]) : -1;
-                    if (counts) top = fmaxf(top, v[q]);
-                }
-            }
-            top = warp_max(top);
-            const bool live = weight != 0.0f && top != -INFINITY;
+            double base = 0.0, mass = 0.0;
+            // (The gradient alone, in place: another CTA may be writing its part of the row already.)
+            const bool live = weight != 0.0f &&
+                              read_entries<T, LOSS, GRAD>(p, z, row, c, Entries{probs + place * p.k, heres + place * p.k, ats + place * p.k, table, r.table},
+                                                          &base, &mass, [&](int col) { return LOSS || slice.owns(col, rank); });
             if (live) {
-                const Slice<T> slice(z, p.vocab, rank, log2_cluster);
-                float part = 0.0f;
-                for (int j0 = lane; j0 < p.k; j0 += 4 * kWarp) {
-                    float v[4];
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const int j = j0 + q * kWarp;
-                        const int col = j < p.k ? at[j] : -1;
-                        // (The gradient alone, in place: another CTA may be writing its part of the row already.)
-                        v[q] = col >= 0 && (LOSS || slice.owns(col, rank)) ? to_f32(z[col]) : 0.0f;
-                        if (col >= 0) part += ex2_approx((prob[j] - top) * c);
-                    }
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        if (j0 + q * kWarp < p.k) here[j0 + q * kWarp] = v[q];
-                    }
-                }
                 if (lane < slice.edges() && (LOSS || rank == 0)) out.edge[lane] = to_f32(z[slice.edge_col(lane, p.vocab)]);
-                const double sum = static_cast<double>(warp_sum(part));
-                const double norm = p.teacher_lse == nullptr ? static_cast<double>(top) * p.inv_temperature + log(sum)
-                                                             : static_cast<double>(p.teacher_lse[row]);
-                double base = 0.0, mass = 0.0;
-                for (int j = lane; j < p.k; j += kWarp) {
-                    float pj = 0.0f;
-                    if (at[j] >= 0) {
-                        const double logp = static_cast<double>(prob[j]) * p.inv_temperature - norm;
-                        pj = expf(static_cast<float>(logp));
-                        if (LOSS && pj != 0.0f) base += pj * (logp - static_cast<double>(here[j]) * p.inv_temperature);
-                        mass += pj;
-                    }
-                    prob[j] = pj;
-                }
-                base = warp_sum(base);
-                mass = warp_sum(mass);
-                if (GRAD) {
-                    // Entries of one column: each entry writes its number into the column's place of a hash table
-                    // and looks who is there.  Another column there: again with another hash (that column's own
-                    // entries are all in the same position); its own column: to be folded.  What the table held
-                    // before does not matter, as a place is read after at least one entry wrote it.
-                    uint32_t pending = 0, same = 0;  // bit q: entry lane + 32 q
-                    for (int j = lane, q = 0; j < p.k; j += kWarp, ++q) pending |= at[j] >= 0 ? 1u << q : 0u;
-                    for (uint32_t round = 0; __any_sync(kFullMask, pending != 0u); ++round) {
-                        const uint32_t mix = 0x9E3779B1u + 2u * round * 0x85EBCA6Bu;  // odd
-                        __syncwarp();
-                        for (uint32_t left = pending; left != 0u; left &= left - 1u) {
-                            const int j = lane + kWarp * (__ffs(left) - 1);
-                            table[(static_cast<uint32_t>(at[j] + 1) * mix >> 15) & (r.table - 1)] = static_cast<uint16_t>(j);
-                        }
-                        __syncwarp();
-                        for (uint32_t left = pending; left != 0u; left &= left - 1u) {
-                            const int q = __ffs(left) - 1, j = lane + kWarp * q;
-                            const int w = table[(static_cast<uint32_t>(at[j] + 1) * mix >> 15) & (r.table - 1)];
-                            if (w == j || at[w] == at[j]) {
-                                pending &= ~(1u << q);
-                                if (w != j) same |= 1u << q;
-                            }
-                        }
-                    }
-                    __syncwarp();
-                    // The first entry of a shared column gets the sum (in entry order over lanes, a fixed tree); the
-                    // others are dropped.
-                    for (uint32_t owners = __ballot_sync(kFullMask, same != 0u); owners != 0u;
-                         owners = __ballot_sync(kFullMask, same != 0u)) {
-                        const int owner = __ffs(owners) - 1;
-                        const int j = __shfl_sync(kFullMask, same != 0u ? lane + kWarp * (__ffs(same) - 1) : 0, owner);
-                        if (lane == owner) same &= same - 1u;
-                        const int col = at[j];
-                        if (col < 0) continue;  // dropped with an earlier one
-                        int least = p.k;
-                        float sum_p = 0.0f;
-                        for (int i = lane; i < p.k; i += kWarp) {
-                            if (at[i] == col) {
-                                least = min(least, i);
-                                sum_p += prob[i];
-                            }
-                        }
-                        least = __reduce_min_sync(kFullMask, least);
-                        sum_p = warp_sum(sum_p);
-                        __syncwarp();
-                        for (int i = lane; i < p.k; i += kWarp) {
-                            if (at[i] == col) {
-                                if (i == least) prob[i] = sum_p;
-                                else at[i] = -1;
-                            }
-                        }
-                        __syncwarp();
-                    }
-                }
                 if (lane == 0) {
                     out.base = base;
                     out.mass = mass;
@@ -640,7 +653,7 @@ distill_ring_kernel(const RingParams r) {
         auto close = [&]() {
             if (!stat_wait(cluster, &stat_full[last.number % kStatSlots], static_cast<uint32_t>(last.number / kStatSlots & 1), failed, r.error_flag)) return false;
             const float2 f = fold_stats(row_of_stats(last.number), cluster * kSumWarps, c);
-            if (rank == 0 && lane == 0) write_loss(p, prepared[last.place], last.row, f);
+            if (rank == 0 && lane == 0) write_loss(p, prepared[last.place].base, prepared[last.place].mass, last.row, f);
             __syncwarp();
             if (lane == 0) mbar_arrive(&prep_empty[last.place]);
             last.row = -1;
@@ -653,10 +666,10 @@ distill_ring_kernel(const RingParams r) {
             if (live) {
                 const T* z = static_cast<const T*>(p.logits) + row * p.logits_stride;
                 const Slice<T> slice(z, p.vocab, rank, log2_cluster);
-                float mx = -INFINITY, s = 0.0f;
+                Running run;
                 bool ok = true;
                 for (int i = 0; i < slice.chunks; ++i, slot.next(r.slots)) {
-                    if (kSumGroups > 1 && (i & 1) != group) continue;
+                    if (kSumGroups > 1 && (slot.place & 1) != group) continue;
                     ok = warp_wait(&full[slot.place], slot.parity, failed, r.error_flag);
                     if (!ok) break;
                     const uint4* chunk = reinterpret_cast<const uint4*>(ring + static_cast<size_t>(slot.place) * kChunkBytes);
@@ -664,45 +677,14 @@ distill_ring_kernel(const RingParams r) {
                     uint4 raw[kBatch];
 #pragma unroll
                     for (int q = 0; q < kBatch; ++q) raw[q] = tg + q * kGroup < n ? chunk[tg + q * kGroup] : lowest_pack(T{});
-                    float big = -INFINITY;
-#pragma unroll
-                    for (int q = 0; q < kBatch; ++q) {
-                        float2 v[N / 2];
-                        unpack2(raw[q], v, T{});
-#pragma unroll
-                        for (int e = 0; e < N / 2; ++e) big = fmaxf(big, fmaxf(v[e].x, v[e].y));
-                    }
-                    const float now = fmaxf(mx, big);
-                    const float ref = now == -INFINITY ? 0.0f : now;  // nothing but -inf so far: exp(-inf) each
-                    const float2 down = both(-ref), c2 = both(c);
-                    float2 add[2] = {both(0.0f), both(0.0f)};
-#pragma unroll
-                    for (int q = 0; q < kBatch; ++q) {
-                        float2 v[N / 2];
-                        unpack2(raw[q], v, T{});
-#pragma unroll
-                        for (int e = 0; e < N / 2; ++e) {
-                            v[e] = mul2(add2(v[e], down), c2);
-                            add[e & 1] = add2(add[e & 1], make_float2(ex2_approx(v[e].x), ex2_approx(v[e].y)));
-                        }
-                    }
-                    const float2 sum = add2(add[0], add[1]);
-                    s = s * exp_diff(mx, now, c) + (sum.x + sum.y);
-                    mx = now;
+                    run.take<T>(raw, c);
                     // The place is given back once every lane's loads have returned, not when they are under way: the
                     // vote needs sums of all of them (a sum is never -1).
-                    if (!GRAD && !__any_sync(kFullMask, s == -1.0f) && lane == 0) mbar_arrive(&empty[slot.place]);
+                    if (!GRAD && !__any_sync(kFullMask, run.s == -1.0f) && lane == 0) mbar_arrive(&empty[slot.place]);
                 }
                 if (!ok) break;
-                if (rank == 0 && w == 0) {
-                    const bool is_edge = lane < slice.edges();
-                    const float v = is_edge ? prepared[prep.place].edge[lane] : -INFINITY;
-                    const float now = fmaxf(mx, v);
-                    s = s * exp_diff(mx, now, c) + (is_edge ? ex2_approx((v - (now == -INFINITY ? 0.0f : now)) * c) : 0.0f);
-                    mx = now;
-                }
-                const float top = warp_max(mx);
-                const float2 mine = make_float2(top, warp_sum(s * exp_diff(mx, top, c)));
+                if (rank == 0 && w == 0 && lane < slice.edges()) run.take_one(prepared[prep.place].edge[lane], c);
+                const float2 mine = run.of_warp(c);
                 uint64_t* bar = &stat_full[live_rows % kStatSlots];
                 if (cluster == 1) {  // launched without a cluster: nothing but the CTA's own shared memory
                     if (lane == 0) {
@@ -748,15 +730,16 @@ distill_ring_kernel(const RingParams r) {
                 if (LOSS) {
                     if (!stat_wait(cluster, &stat_full[live_rows % kStatSlots], static_cast<uint32_t>(live_rows / kStatSlots & 1), failed, r.error_flag)) break;
                     f = fold_stats(&stat[live_rows % kStatSlots][0], cluster * kSumWarps, c);
-                    if (rank == 0 && w == 0 && lane == 0) write_loss(p, pre, row, f);
+                    if (rank == 0 && w == 0 && lane == 0) write_loss(p, pre.base, pre.mass, row, f);
                     ++live_rows;
                 }
                 const float m = f.x, total = f.y, coef = scale * pre.weight;
                 const float mass = p.teacher_lse == nullptr && pre.mass == pre.mass ? 1.0f : static_cast<float>(pre.mass);
                 const float each = coef * mass / total;
+                const int start = slot.place;
                 bool ok = true;
                 for (int i = 0; i < slice.chunks; ++i, slot.next(r.slots)) {
-                    if (kWriteGroups > 1 && (i & 1) != group) continue;
+                    if (kWriteGroups > 1 && (slot.place & 1) != group) continue;
                     ok = warp_wait(&full[slot.place], slot.parity, failed, r.error_flag);
                     if (!ok) break;
                     const unsigned char* chunk = ring + static_cast<size_t>(slot.place) * kChunkBytes;
@@ -804,7 +787,7 @@ distill_ring_kernel(const RingParams r) {
                     if (slice.inner(col)) {
                         const int pack = (col - slice.head) / N - slice.lo, in = pack % kChunkPacks;
                         owner = (same_phase ? in : in * N + (col - slice.head) % N) % kGroup / kWarp;
-                        if (kWriteGroups > 1) owner += pack / kChunkPacks % 2 * kGroupWarps;
+                        if (kWriteGroups > 1) owner += ((start + pack / kChunkPacks) % r.slots & 1) * kGroupWarps;
                     }
                     if (owner != w) continue;
                     const float q = ex2_approx((heres[prep.place * p.k + j] - m) * c) / total;
@@ -836,9 +819,10 @@ distill_mean_kernel(const float* row_loss, const float* row_weight, int64_t rows
     __shared__ double red[1024 / kWarp];
     pdl_wait();
     double s = 0.0;
+#pragma unroll 8
     for (int64_t r = threadIdx.x; r < rows; r += blockDim.x) {
-        const float w = row_weight == nullptr ? 1.0f : row_weight[r];
-        if (w != 0.0f) s += static_cast<double>(w) * row_loss[r];
+        const float w = row_weight == nullptr ? 1.0f : row_weight[r], loss = row_loss[r];
+        s += w != 0.0f ? static_cast<double>(w) * loss : 0.0;
     }
     s = warp_sum(s);
     if ((threadIdx.x & (kWarp - 1)) == 0) red[threadIdx.x / kWarp] = s;
@@ -907,8 +891,21 @@ int launch_ring(const DistillParams& p, const DeviceInfo* info, int cluster, int
                      dim3(static_cast<unsigned int>(cluster), 1, 1), tuning().pdl != 0, r);
 }
 
-// Rows of at least this many bytes take the ring form.
-constexpr int64_t kRingFromBytes = 16384;
+// Rows of more than this many bytes take the ring form: what eight warps hold.
+constexpr int64_t kRingFromBytes = 8 * kWarp * kHeld * 16;
+
+template <class T, bool LOSS, bool GRAD, int WARPS, int HELD>
+int launch_held(const DistillParams& p, int places, cudaStream_t stream) {
+    constexpr int teams = WARPS == 1 ? 256 / kWarp : 1;
+    const size_t smem = static_cast<size_t>(teams) * (static_cast<size_t>(p.k) * 12 + static_cast<size_t>(places) * 2);
+    auto kernel = distill_rows_kernel<T, LOSS, GRAD, WARPS, HELD>;
+    if (smem > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+        if (e != cudaSuccess) return static_cast<int>(e);
+    }
+    return launch_ex(kernel, dim3(static_cast<unsigned int>(ceil_div(p.rows, teams))), dim3(teams * WARPS * kWarp), smem, stream,
+                     dim3(1, 1, 1), tuning().pdl != 0, p, places);
+}
 
 template <bool LOSS, bool GRAD>
 int launch_rows(const DistillParams& p, int dtype, cudaStream_t stream) {
@@ -916,9 +913,9 @@ int launch_rows(const DistillParams& p, int dtype, cudaStream_t stream) {
     const DeviceInfo* info = current_device_info(&status);
     if (info == nullptr) return status;
     const int64_t bytes = static_cast<int64_t>(p.vocab) * static_cast<int64_t>(dtype_bytes(dtype));
-    if (bytes >= kRingFromBytes) {
-        int table = 64;
-        while (table < 2 * p.k) table *= 2;
+    int table = 64;
+    while (table < 2 * p.k) table *= 2;
+    if (bytes > kRingFromBytes) {
         const int64_t entries = static_cast<int64_t>(kPrepSlots) * p.k * 12 + kPrepWarps * 2 * table;
         int64_t slots = (kRingSmem - entries) / kChunkBytes;
         if (slots > kMaxSlots) slots = kMaxSlots;
@@ -940,11 +937,14 @@ int launch_rows(const DistillParams& p, int dtype, cudaStream_t stream) {
         status = launch_rows<true, false>(p, dtype, stream);
         return status != FDL_OK ? status : launch_rows<false, true>(p, dtype, stream);
     }
-    const int grid = persistent_grid(info, 16, p.rows);
     return with_dtype(dtype, [&](auto* tag) {
         using T = std::remove_pointer_t<decltype(tag)>;
-        return launch_ex(distill_rows_kernel<T, LOSS, GRAD>, dim3(grid), dim3(kRowThreads), 0, stream, dim3(1, 1, 1),
-                         tuning().pdl != 0, p);
+        constexpr int64_t warp_bytes = kWarp * kHeld * 16;
+        if (bytes <= warp_bytes / 2) return launch_held<T, LOSS, GRAD, 1, kHeld / 2>(p, table, stream);
+        if (bytes <= warp_bytes) return launch_held<T, LOSS, GRAD, 1, kHeld>(p, table, stream);
+        if (bytes <= 2 * warp_bytes) return launch_held<T, LOSS, GRAD, 2, kHeld>(p, table, stream);
+        if (bytes <= 4 * warp_bytes) return launch_held<T, LOSS, GRAD, 4, kHeld>(p, table, stream);
+        return launch_held<T, LOSS, GRAD, 8, kHeld>(p, table, stream);
     });
 }
 

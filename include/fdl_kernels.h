@@ -416,7 +416,7 @@ int fdl_normal_f32(float* data, int64_t n, float mean, float stddev, uint64_t se
  * with log sum exp of ALL its logits / T -- and q = softmax(logits / T):
  *   row_loss[r] = sum_j p_j (log p_j - log q[index_j]),  loss[0] = scale * sum_r row_weight_r * row_loss_r.
  * A column may be named by several entries.  A row of weight 0, or in which no entry counts, is left
- * out: its loss is 0 and its logits are not read.  row_weight NULL: 1 for each row.  A student logit
+ * out: its loss is 0, whatever its logits hold.  row_weight NULL: 1 for each row.  A student logit
  * of -inf at a place where p_j > 0 makes the row's loss +inf; a row of nothing but -inf, and NaN or
  * +inf among its logits, make it NaN.  row_stats: [rows, 2], the row's largest logit m and
  * sum exp((logits - m) / T) (0, 0 for a row left out); the backward call takes it.
