@@ -569,10 +569,10 @@ def verify_draft(target, draft_tokens, accept_u, sample_u, draft=None, draft_len
     vocab = target.shape[2]
     target_batch, target_row, within = target.stride()
     draft_batch = draft_row = 0
+    within_draft = 1
     if draft is not None:
         draft_batch, draft_row, within_draft = draft.stride()
-        within = max(within, within_draft)
-    if vocab > 1 and within != 1:
+    if vocab > 1 and not (within == within_draft == 1):
         raise ValueError(f"{where}: expected a contiguous last dimension")
     tokens = _torch.empty((batch, drafted + 1), dtype=i64, device=target.device)
     accepted = _torch.empty((batch,), dtype=i64, device=target.device)

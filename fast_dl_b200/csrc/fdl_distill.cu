@@ -10,6 +10,7 @@
 //
 // Differences of logarithms are taken in 64 bits (k of them a row): where teacher and student
 // agree, the loss is a small difference of numbers of size ten.
+#include <atomic>
 #include <climits>
 #include <type_traits>
 
@@ -194,20 +195,38 @@ __device__ __forceinline__ uint4 lowest_pack(float) { return make_uint4(0xff8000
 __device__ __forceinline__ uint4 lowest_pack(__half) { return make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u); }
 __device__ __forceinline__ uint4 lowest_pack(__nv_bfloat16) { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
 
+// The largest element of some packs (NaN is passed over); 16-bit types two at a time, before they are unpacked.
+template <int PACKS>
+__device__ __forceinline__ float packs_max(const uint4 (&raw)[PACKS], float) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int q = 0; q < PACKS; ++q) {
+        m = fmaxf(m, fmaxf(fmaxf(__uint_as_float(raw[q].x), __uint_as_float(raw[q].y)),
+                           fmaxf(__uint_as_float(raw[q].z), __uint_as_float(raw[q].w))));
+    }
+    return m;
+}
+template <int PACKS, class T>
+__device__ __forceinline__ float packs_max(const uint4 (&raw)[PACKS], T) {
+    using Pair = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+    const uint4 low = lowest_pack(T{});
+    Pair m = *reinterpret_cast<const Pair*>(&low.x);
+#pragma unroll
+    for (int q = 0; q < PACKS; ++q) {
+        const Pair a = __hmax2(*reinterpret_cast<const Pair*>(&raw[q].x), *reinterpret_cast<const Pair*>(&raw[q].y));
+        const Pair b = __hmax2(*reinterpret_cast<const Pair*>(&raw[q].z), *reinterpret_cast<const Pair*>(&raw[q].w));
+        m = __hmax2(m, __hmax2(a, b));
+    }
+    return fmaxf(to_f32(m.x), to_f32(m.y));
+}
+
 // A running maximum and sum of exponentials relative to it.
 struct Running {
     float m = -INFINITY, s = 0.0f;
     template <class T, int PACKS>
     __device__ __forceinline__ void take(const uint4 (&raw)[PACKS], float c) {
         constexpr int M = kPack<T> / 2;
-        float big = -INFINITY;
-#pragma unroll
-        for (int q = 0; q < PACKS; ++q) {
-            float2 v[M];
-            unpack2(raw[q], v, T{});
-#pragma unroll
-            for (int e = 0; e < M; ++e) big = fmaxf(big, fmaxf(v[e].x, v[e].y));
-        }
+        const float big = packs_max(raw, T{});
         const float now = fmaxf(m, big);
         const float ref = now == -INFINITY ? 0.0f : now;  // nothing but -inf so far: exp(-inf) each
         const float2 down = both(-ref), c2 = both(c);
@@ -846,15 +865,15 @@ int check_common(const void* logits, int64_t stride, int dtype, const void* teac
 
 // Clusters of `cluster` ring CTAs that fit the device at once (asked once for each kernel, size and device).
 template <class K>
-int active_clusters(K kernel, int* cache, const DeviceInfo* info, int cluster, size_t smem, int* out) {
+int active_clusters(K kernel, std::atomic<int>* cache, const DeviceInfo* info, int cluster, size_t smem, int* out) {
     if (cluster == 1) {
         *out = info->sm_count;
         return FDL_OK;
     }
     int log2 = 0;
     while ((1 << log2) < cluster) ++log2;
-    int& known = cache[(info->device % kMaxDevicesTracked) * 4 + log2];
-    if (known == 0) {
+    std::atomic<int>& known = cache[(info->device % kMaxDevicesTracked) * 4 + log2];
+    if (known.load() == 0) {
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(static_cast<unsigned int>(info->sm_count / cluster * cluster));
         cfg.blockDim = dim3(kRingThreads);
@@ -868,15 +887,15 @@ int active_clusters(K kernel, int* cache, const DeviceInfo* info, int cluster, s
         int n = 0;
         const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
         if (e != cudaSuccess) return static_cast<int>(e);
-        known = n < 1 ? 1 : n;
+        known.store(n < 1 ? 1 : n);
     }
-    *out = known;
+    *out = known.load();
     return FDL_OK;
 }
 
 template <class T, bool LOSS, bool GRAD>
 int launch_ring(const DistillParams& p, const DeviceInfo* info, int cluster, int slots, int table, cudaStream_t stream) {
-    static int cache[kMaxDevicesTracked * 4] = {};
+    static std::atomic<int> cache[kMaxDevicesTracked * 4] = {};
     auto kernel = distill_ring_kernel<T, LOSS, GRAD>;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem);
     if (e != cudaSuccess) return static_cast<int>(e);
@@ -899,8 +918,8 @@ int launch_held(const DistillParams& p, int places, cudaStream_t stream) {
     constexpr int teams = WARPS == 1 ? 256 / kWarp : 1;
     const size_t smem = static_cast<size_t>(teams) * (static_cast<size_t>(p.k) * 12 + static_cast<size_t>(places) * 2);
     auto kernel = distill_rows_kernel<T, LOSS, GRAD, WARPS, HELD>;
-    if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (smem > 48 * 1024) {  // (the most that a call takes, not this one's: another thread may be between its own two calls)
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, teams * kMaxEntries * 16);
         if (e != cudaSuccess) return static_cast<int>(e);
     }
     return launch_ex(kernel, dim3(static_cast<unsigned int>(ceil_div(p.rows, teams))), dim3(teams * WARPS * kWarp), smem, stream,

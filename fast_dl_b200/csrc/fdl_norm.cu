@@ -501,6 +501,7 @@ norm_residual_backward_kernel(const NormParams p) {
 // scale and a shared gate); a thread reads and writes only its own columns of them, so no barrier guards them.
 
 constexpr int kMaxStages = 4;
+constexpr int kRingRoom = 227 * 1024 - 4096;  // dynamic shared memory of a CTA alone on its SM
 
 struct RingPlan {
     int stages;
@@ -1602,7 +1603,7 @@ RingShape ring_shape(int64_t cols, int dtype, int tiles, int weights, bool backw
     const size_t fixed = static_cast<size_t>(r.plan.weights) * 4 * weights;
     const size_t stage = static_cast<size_t>(r.plan.tile) * 16 * tiles;
     for (; r.blocks >= 1; --r.blocks) {  // fewer CTAs where less than two stages would fit
-        const size_t room = static_cast<size_t>(227 * 1024) / r.blocks - 4096;
+        const size_t room = static_cast<size_t>(kRingRoom + 4096) / r.blocks - 4096;
         if (room < fixed + 2 * stage) continue;
         const size_t most = (room - fixed) / stage;
         r.plan.stages = most > kMaxStages ? kMaxStages : static_cast<int>(most);
@@ -1704,7 +1705,8 @@ int launch_direct(bool backward, int dtype, bool vec, const NormParams& p, const
 
 template <class K, class... Args>
 int launch_ring(K kernel, const NormParams& p, const RingShape& r, int64_t grid, cudaStream_t stream) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(r.smem));
+    // (the most that a shape takes, not this one's: another thread may be between its own two calls)
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingRoom);
     if (e != cudaSuccess) return static_cast<int>(e);
     return launch_ex(kernel, dim3(static_cast<unsigned int>(grid)), dim3(r.threads), r.smem, stream, dim3(r.cluster, 1, 1),
                      tuning().pdl != 0, p, r.plan);

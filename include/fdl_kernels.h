@@ -405,7 +405,11 @@ int fdl_normal_f32(float* data, int64_t n, float mean, float stddev, uint64_t se
  * These entry points take tensors of the type `dtype` (enum fdl_dtype); gamma, beta, statistics,
  * losses and random numbers are float.  Arithmetic is in 32 bits or more, a result of 16 bits is
  * rounded once, to nearest even.  They use no library workspace: calls on different streams may
- * overlap, and a captured call holds on to nothing but the caller's buffers. */
+ * overlap, and a captured call holds on to nothing but the caller's buffers.  (Make the first call of
+ * a process outside a capture: it sets up the error word that fdl_take_device_error reads, which the
+ * kernels that wait for their bulk copies or for the CTAs of their cluster report to.)  The bits of a
+ * result do not depend on what else runs, but a row's may differ by roundings with the number of
+ * rows in the call, which decides how a row is dealt out. */
 
 /* Distillation from the teacher's k highest logits.  logits: [rows, vocab] of the student, rows
  * `logits_stride` elements apart (>= vocab; columns beyond vocab are neither read nor written);

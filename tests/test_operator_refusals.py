@@ -140,7 +140,9 @@ def test_binding_refuses_wrong_shapes_types_and_strides(fdl, cuda):
            lambda: fdl.verify_draft(torch.zeros(4, 4, 9, device="cuda"), i, t, t[:, 0]),
            lambda: fdl.verify_draft(torch.zeros(4, 9, 4, device="cuda").transpose(1, 2), i, t, t[:, 0].contiguous()),
            lambda: fdl.verify_draft(torch.zeros(4, 4, 9, device="cuda"), i, t, t[:, 0].contiguous(),
-                                    draft=torch.zeros(4, 3, 9, device="cuda").half())]
+                                    draft=torch.zeros(4, 3, 9, device="cuda").half()),
+           lambda: fdl.verify_draft(torch.zeros(4, 4, 9, device="cuda"), i, t, t[:, 0].contiguous(),
+                                    draft=torch.zeros(4, 3, 1, device="cuda").expand(4, 3, 9))]
     for k, fn in enumerate(bad):
         with pytest.raises(ValueError):
             fn()
