@@ -10,6 +10,11 @@
 //
 // Differences of logarithms are taken in 64 bits (k of them a row): where teacher and student
 // agree, the loss is a small difference of numbers of size ten.
+//
+// What bounds it: a row has to be read once for the loss, and written once more for the gradient; loss and gradient
+// in one call keep the row on chip between the two.  Measured on B200 (floors at 6548 GB/s in brackets): loss and
+// gradient of [4096, 65537] f32 360 us [321], of [2048, 131072] bf16 225 us [160], of [15660, 966] f16 33 us [10],
+// gradient of [1000, 50257] f32 78 us [60], loss of [8, 32000] f32 7.7 us with its mean.
 #include <atomic>
 #include <climits>
 #include <type_traits>
@@ -414,6 +419,13 @@ distill_rows_kernel(const DistillParams p, int places) {
 // only, so whoever waits for a place has to wait for each of its rounds: with the chunks of a row dealt out in
 // turn, a group could be two rounds ahead of a slow copy and take the place's last chunk for its next.)
 // The elements of a row outside its 16-byte grid (its first and last few) go by plain loads.
+//
+// Of [2048, 131072] bf16's 225 us, 113 are the special-function unit's (two exponentials an element, 16 a cycle and
+// SM; without those of the writes it takes 180 us, without any 174), the rest of the gap to 160 is the chain of a
+// row: its last chunk's copy, sum and exchange.  Measured and dropped: one kind of worker for sums and writes 253
+// us (f32 401), groups of four warps 231, three groups of eight 212-230 (f32 348-366), chunks of 8 KiB 255 and of 18 to
+// 32 KiB 206-246 (f32 367-459), a prefetch of the row into L2 216 (f32 356), half of the writes' exponentials by a
+// polynomial 230, clusters of four where two do (132 of 148 SMs at one CTA an SM).
 //
 // Every wait has a limit; one that gives up ends all of them (and is reported through the error flag).
 

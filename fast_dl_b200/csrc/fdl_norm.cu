@@ -20,6 +20,10 @@
 // row that its team takes, so gamma and beta are read once, and the backward pass's sums over rows grow
 // in registers; each team leaves one partial row of them in scratch, which a second kernel adds in a
 // fixed order (no atomics: the same bits in every run).
+//
+// Measured on B200 (floors at 6548 GB/s in brackets): forward [16384, 4096] bf16 with a full sigmoid gate 126 us [103],
+// [56548, 128] bf16 16 us [11], one row of 4096 4.9 us; backward [16384, 8192] bf16 with a gate for each of 8 runs of
+// rows 313 us [246], [16384, 4096] 159 us [123], [2049, 1001] f32 25 us [8], of which the second kernel is about 5.
 #include <climits>
 #include <initializer_list>
 #include <type_traits>
@@ -495,7 +499,9 @@ norm_residual_backward_kernel(const NormParams p) {
 //
 // For more rows than teams, on the 16-byte grid: one thread asks for whole row slices with bulk-async
 // copies, a few rows ahead of the row that the CTA works on, so the bytes in flight depend on neither
-// registers nor barriers.  Arithmetic goes two floats an instruction: the kernels are near the issue limit.
+// registers nor barriers (loads into registers took 337 us forward and 1289 backward where this form takes 126 and
+// 313).  What bounds it then is the row's chain of sums -- shuffles, a barrier, shuffles -- and the issue of some 40
+// instructions an element pair: 61% of issue slots are busy forward, 48% backward, DRAM half of the time.  Arithmetic goes two floats an instruction: the kernels are near the issue limit.
 // Forward, gamma and beta come from L1 row by row (in shared memory they would take the place of a CTA).
 // Backward, with half the threads an SM, they lie in shared memory as floats (post_gamma times the block's
 // scale and a shared gate); a thread reads and writes only its own columns of them, so no barrier guards them.
