@@ -92,7 +92,8 @@ def make(rows, vocab, k, kind, seed=0, stride=None, tail=False, teacher_kind=Non
 
 
 SHAPES = [(1, 1, 1), (1, 7, 3), (3, 33, 33), (5, 1000, 8), (2, 1027, 64), (9, 4099, 5), (4, 16384, 100), (2, 50257, 128),
-          (1, 131072, 1024), (3, 100003, 17), (700, 129, 4), (2, 262145, 33), (160, 9001, 12), (400, 16385, 40), (90, 40000, 3)]
+          (1, 131072, 1024), (3, 100003, 17), (700, 129, 4), (2, 262145, 33), (160, 9001, 12), (400, 16385, 40), (90, 40000, 3), (2, 400001, 30),
+          (1, 1000003, 5), (20, 1024, 9), (11, 2049, 1), (300, 512, 7)]
 
 
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
