@@ -23,7 +23,7 @@
 //
 // Measured on B200 (floors at 6548 GB/s in brackets): forward [16384, 4096] bf16 with a full sigmoid gate 126 us [103],
 // [56548, 128] bf16 16 us [11], one row of 4096 4.9 us; backward [16384, 8192] bf16 with a gate for each of 8 runs of
-// rows 313 us [246], [16384, 4096] 159 us [123], [2049, 1001] f32 25 us [8], of which the second kernel is about 5.
+// rows 313 us [246], [16384, 4096] 159 us [123], [2049, 1001] f32 24 us [8], of which the second kernel is about 5.
 #include <climits>
 #include <initializer_list>
 #include <type_traits>
